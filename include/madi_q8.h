@@ -336,6 +336,94 @@ int madi_q8_emb_pe_rows(float *out, const void *qs, const void *scales, const ui
 int madi_flash_enc_f16(void *out, const void *q, const void *k, const void *v, uint32_t seq_len,
                        uint32_t nh);
 
+/* ---- 4-bit key/value cache --------------------------------------------------- */
+/* No counterpart in the reference, whose decoder caches K and V in f32
+ * (gemv_q8_qkv's kc and vc) and f16: K and V rows held in 4 bits, 4.5 with
+ * their scales, and the attention that reads them.
+ *
+ * A block is 32 elements x of one head's row (elements 32b..32b+31):
+ *   scale s = min(f16(f32(max|x| / 7)), 9352)
+ *   code  q = sign(x) * min(7, floor(|x| / s + 1/2)), 0 where s = 0
+ * and stands for q * s.  The border between two codes is decided exactly (no
+ * rounded quotient).  Every value held is a finite f16 number at most 65464
+ * (7 * 9352) large: an infinity is held as 7 s, a NaN as 0, so that neither
+ * reaches a row that does not see it.
+ *
+ * A cache is a pool of pages; a page holds `page` tokens of every kv head.
+ * Page p, head h starts at byte (p * nkv + h) * page * d * 9/8 of data; there
+ * (nb = d / 32 blocks, codes as nibbles q + 8):
+ *   K      page * d/2 bytes: token t's row at t * d/2; word (g, b) of the row
+ *          (g < 4) at (g * nb + b) * 4 holds elements 32b + 8g + 0..7, element
+ *          2j in nibble j and element 2j+1 in nibble 4+j
+ *   V      page * d/2 bytes: tokens 4u..4u+3 at u * 2d; word (c, b) (c < 16) at
+ *          (c * nb + b) * 4 holds elements 32b + c (low nibbles) and 32b+16+c
+ *          (high nibbles), its bytes tokens 4u, 4u+2, 4u+1, 4u+3
+ *   scales page * d/8 bytes: tokens 4u..4u+3 at u * d/2; f16 (x, b, t) at
+ *          ((x * nb + b) * 4 + t) * 2, x = 0 for K and 1 for V, t the token - 4u
+ * d is 64, 96, 128 or 256; page a power of two, at least 16; data 16-byte
+ * aligned.  madi_kv4_bytes gives the size of data (0 for a shape it does not take). */
+typedef struct {
+  void *data;       /* device */
+  uint32_t n_pages; /* pages in the pool */
+  uint32_t page;    /* tokens of a page */
+  uint32_t nkv;     /* kv heads */
+  uint32_t d;       /* elements of a head */
+} madi_kv4;
+
+/* The sequences and rows of one call.  Sequence i holds lens[i] tokens (its new
+ * ones included) on the pages table[i * max_pages + 0, 1, ..]; a length past
+ * the table's reach (max_pages * page) counts as that reach.  Its rows are the
+ * last ones: row r of rows_i is position lens[i] - rows_i + r.  rows_i is
+ * `rows` for every i and its rows start at row i * rows of the inputs and
+ * outputs (row_off NULL; then m = b * rows), or row_off[i + 1] - row_off[i],
+ * starting at row row_off[i]; a row at m or beyond, or past the first `rows` of its
+ * sequence, is not read or written, nor is any row before row_off[0] or from row_off[b]
+ * on.  A page number of n_pages or more stands for a page that is not there
+ * (given up by a sliding window): a store leaves out its rows, a load gives
+ * zeros, attention does not see its keys.  Pages may be shared by sequences
+ * except where a store writes them.  The struct itself lies in host memory and
+ * is read during the call; table, lens and row_off on the device when the kernel runs.
+ * len_max is a hint (the longest length to plan the split for; 0: max_pages * page),
+ * and work (16-byte aligned) is where an attention that splits long caches over
+ * workgroups keeps its partial results: with fewer bytes than
+ * madi_kv4_attn_bytes asks for it splits less, without any it does not split.
+ * Calls that may overlap (replays of two graphs, two streams) need a work of
+ * their own each; nothing else is shared between calls. */
+typedef struct {
+  const uint32_t *table;   /* device, [b][max_pages] */
+  const uint32_t *lens;    /* device, [b] */
+  const uint32_t *row_off; /* device, [b + 1], or NULL */
+  uint32_t b, max_pages, rows, m, len_max;
+  void *work;              /* device, or NULL */
+  size_t work_bytes;
+} madi_kv4_batch;
+
+#define MADI_F16 0
+#define MADI_F32 1
+
+size_t madi_kv4_bytes(uint32_t n_pages, uint32_t page, uint32_t nkv, uint32_t d);
+/* Quantise the rows k, v [m][nkv * d] (rows ldk and ldv elements apart) into
+ * the cache.  Rows 16-byte aligned.  Rows at a position below 0 are left out. */
+int madi_kv4_store(const madi_kv4 *cache, const madi_kv4_batch *batch, const void *k, const void *v,
+                   uint32_t ldk, uint32_t ldv, int dtype);
+/* Read them back: k, v = q * s rounded once to dtype, zeros at a position below 0. */
+int madi_kv4_load(void *k, void *v, uint32_t ldk, uint32_t ldv, int dtype, const madi_kv4 *cache,
+                  const madi_kv4_batch *batch);
+/* Attention over the cache: out[row][head] = softmax(scale * q . K^T) . V over the
+ * keys that the row sees, nh query heads in nh / nkv consecutive ones per kv
+ * head, q and out [m][nh * d] (rows ldq and ldo elements apart, 16-byte
+ * aligned).  causal: the row at position p sees positions j <= p and, where window
+ * is not 0, j > p - window; not causal (cross-attention): all lens[i] of them,
+ * window 0.  A row that sees no key becomes zeros.  Scores, softmax and sums
+ * are f32.  With f16 rows the probabilities and V values enter the product as
+ * f16; with f32 rows every operand is kept to 22 bits or more.  out may be q
+ * itself (same rows), else it must not overlap it. */
+int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, const madi_kv4_batch *batch,
+                  uint32_t nh, uint32_t ldo, uint32_t ldq, uint32_t window, int causal, int dtype,
+                  float scale);
+/* Bytes of work with which madi_kv4_attn splits as it sees fit (host only). */
+size_t madi_kv4_attn_bytes(const madi_kv4 *cache, const madi_kv4_batch *batch, uint32_t nh);
+
 #ifdef __cplusplus
 }
 #endif

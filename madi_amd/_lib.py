@@ -19,6 +19,7 @@ ERRORS = {
     -9: "MADI_ERR_ARG",
 }
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RES = 0, 1, 2, 3
+F16, F32 = 0, 1
 
 _P = ctypes.c_void_p
 _U32 = ctypes.c_uint32
@@ -69,6 +70,11 @@ SIGNATURES = {
     "madi_q8_emb_lookup_indirect": (_I, [_P, _P, _P, _P, _P, _U32, _U32]),
     "madi_q8_emb_pe_rows": (_I, [_P, _P, _P, _P, _P, _U32, _U32, _U32, _U32]),
     "madi_flash_enc_f16": (_I, [_P, _P, _P, _P, _U32, _U32]),
+    "madi_kv4_bytes": (_SZ, [_U32, _U32, _U32, _U32]),
+    "madi_kv4_store": (_I, [_P, _P, _P, _P, _U32, _U32, _I]),
+    "madi_kv4_load": (_I, [_P, _P, _U32, _U32, _I, _P, _P]),
+    "madi_kv4_attn": (_I, [_P, _P, _P, _P, _U32, _U32, _U32, _U32, _I, _I, ctypes.c_float]),
+    "madi_kv4_attn_bytes": (_SZ, [_P, _P, _U32]),
 }
 
 

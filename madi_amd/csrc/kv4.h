@@ -1,0 +1,66 @@
+// kv4.h -- the 4-bit key/value cache's layout (see madi_q8.h) and the checks
+// that its entry points share.
+#pragma once
+
+#include "common.h"
+
+namespace madi {
+
+// What a kernel needs of a madi_kv4 and a madi_kv4_batch.
+struct Kv4Args {
+  uint8_t *data;
+  const uint32_t *table, *lens, *row_off;
+  uint32_t n_pages, shift, nkv, max_pages, rows, m;
+};
+
+// Checks of the structs, the same for every entry point; fills `a`.
+int kv4_args(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, Kv4Args *a);
+// Checks rows of `width` elements of dtype `ld` apart at p, and tells their
+// extent in bytes.
+int kv4_rows(const char *what, const char *name, const void *p, uint32_t m, uint64_t width,
+             uint32_t ld, int dtype, size_t *bytes);
+inline size_t kv4_cache_bytes(const madi_kv4 *c) {
+  return madi_kv4_bytes(c->n_pages, c->page, c->nkv, c->d);
+}
+inline bool kv4_overlap(const void *a, size_t an, const void *b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return an && bn && x < y + bn && y < x + an;
+}
+
+// ---------------------------------------------------------------- device side
+// One sequence of the batch: its length, its rows [row0, row0 + nrows) of the
+// inputs and outputs, and the position of the first.
+struct Kv4Seq {
+  int32_t len, pos0;
+  uint32_t row0, nrows;
+};
+__device__ inline Kv4Seq kv4_seq(const Kv4Args &a, uint32_t i) {
+  Kv4Seq s;
+  const uint32_t reach = a.max_pages << a.shift, len = a.lens[i];
+  s.len = (int32_t)(len < reach ? len : reach);
+  uint32_t lo = i * a.rows, hi = lo + a.rows;
+  if (a.row_off) {
+    lo = a.row_off[i];
+    hi = a.row_off[i + 1];
+  }
+  hi = hi < a.m ? hi : a.m;
+  lo = lo < hi ? lo : hi;
+  s.row0 = lo;
+  s.nrows = hi - lo;
+  s.pos0 = s.len - (int32_t)s.nrows;
+  s.nrows = s.nrows < a.rows ? s.nrows : a.rows;
+  return s;
+}
+// Page of position pos (0 <= pos < reach) of sequence i.
+__device__ inline uint32_t kv4_page(const Kv4Args &a, uint32_t i, uint32_t pos) {
+  return a.table[(size_t)i * a.max_pages + (pos >> a.shift)];
+}
+// Bytes of one page and head, and the start of page p, head h.
+__device__ inline size_t kv4_block_bytes(uint32_t shift, uint32_t d) {
+  return ((size_t)d * 9 / 8) << shift;
+}
+__device__ inline uint8_t *kv4_block(const Kv4Args &a, uint32_t p, uint32_t h, uint32_t d) {
+  return a.data + ((size_t)p * a.nkv + h) * kv4_block_bytes(a.shift, d);
+}
+
+}  // namespace madi

@@ -1,0 +1,550 @@
+// kv4_attn.hip -- attention over the 4-bit key/value cache (madi_kv4_attn; the
+// format and the layout are in madi_q8.h).
+//
+// The query heads of a kv head and the rows of a sequence make the columns of
+// the products: column c is row c / G, head c % G of the G = nh / nkv.  A wave
+// takes 16 columns and walks the keys 32 at a time:
+//   S^T = K Q^T, v_mfma_f32_16x16x32_f16 with 16 keys as rows and one 32-element
+//     block as K: lane (g, r) passes row r's word (g, b) as eight f16 codes, and the
+//     block's sum gets its key's scale in f32: S = sum_b s_b (Q K^T)_b.  (Codes
+//     masked into f16 subnormals would need no bias taken off, but the matrix
+//     core sums products of subnormals to 2^-18 only, against 2^-24.)
+//   softmax over a running reference that is raised only when a score passes
+//     it by 2^8, so most steps exchange nothing between lanes.
+//   O^T += V^T P^T, 32 keys as K and 16 elements as rows: P^T comes straight
+//     from the S^T registers (lane (g, c) holds keys 4g..4g+3 of both tiles),
+//     V as (n - 8) s in f16 from the words that hold four tokens.
+// f32 rows: q, P and V are each split in two f16 (22 bits; V's 15 bits exactly),
+// the products with both low parts left out (2^-22).
+#include "kv4.h"
+
+using namespace madi;
+
+namespace {
+
+constexpr int kCols = 16;  // columns of a wave (MFMA columns)
+constexpr int kKeys = 32;  // keys of a step
+constexpr float kNever = -1e30f;  // reference before any key was seen
+// P is 2^(x - M) with M at first the largest x - 7, raised when an x passes M
+// by 15: P at most 2^15 (f16 holds 2^16), and a P that rounds to nothing is
+// 2^-32 of the largest.
+constexpr float kLift = 7.0f, kRaise = 15.0f;
+
+struct AttnArgs {
+  Kv4Args kv;
+  const void *q;
+  void *out;
+  float *work;
+  uint32_t ldq, ldo, group, window, causal, splits, min_steps;
+  float scale;
+};
+
+template <int N>
+__device__ inline void load_words(const uint8_t *p, uint32_t (&w)[N]) {
+  constexpr int A = N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4;
+  __builtin_memcpy(w, __builtin_assume_aligned(p, A), 4 * N);
+}
+__device__ inline f16x2 as_f16x2(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+__device__ inline uint32_t as_u32(f16x2 v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ inline f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(f16x8, (u32x4){a, b, c, d});
+}
+__device__ inline f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// over the four lanes that share a column
+__device__ inline void swap16(float v, float &x, float &y) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = __builtin_bit_cast(float, (uint32_t)s[0]);
+  y = __builtin_bit_cast(float, (uint32_t)s[1]);
+}
+__device__ inline void swap32(float v, float &x, float &y) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  x = __builtin_bit_cast(float, (uint32_t)s[0]);
+  y = __builtin_bit_cast(float, (uint32_t)s[1]);
+}
+__device__ inline float sum_across(float v) {
+  float x, y;
+  swap16(v, x, y);
+  swap32(x + y, x, y);
+  return x + y;
+}
+__device__ inline float max_across(float v) {
+  float x, y;
+  swap16(v, x, y);
+  swap32(__builtin_fmaxf(x, y), x, y);
+  return __builtin_fmaxf(x, y);
+}
+
+// One step's 32 keys as they lie in the cache, and whether their pages exist.
+template <int NB>
+struct Step {
+  uint32_t k[2][NB], v[2][NB];
+  uint32_t ks[2][2 * NB], vs[2][2 * NB];  // f16 [block][4 tokens]
+  bool there[2];
+};
+
+template <int NB>
+__device__ inline void fetch(Step<NB> &t, const Kv4Args &a, uint32_t seq, uint32_t head, int32_t key,
+                             int32_t len, uint32_t lane) {
+  constexpr uint32_t D = NB * 32;
+  const uint32_t r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // a tile past the end has no page entry to read: any valid one stands in
+    const int32_t at = key + 16 * i;
+    uint32_t page = 0xffffffffu;
+    if (at < len) page = kv4_page(a, seq, at);
+    t.there[i] = page < a.n_pages;
+    if (!t.there[i]) page = 0;
+    const uint32_t off = (uint32_t)at & ((1u << a.shift) - 1);
+    const uint8_t *blk = kv4_block(a, page, head, D);
+    const uint8_t *kp = blk + (size_t)(off + r) * (D / 2) + g * (4 * NB);
+    const uint8_t *vp = blk + ((size_t)(D / 2) << a.shift) + (size_t)(off / 4 + g) * (2 * D) + r * (4 * NB);
+    const uint8_t *sp = blk + ((size_t)D << a.shift) + (size_t)(off / 4 + g) * (D / 2);
+    load_words<NB>(kp, t.k[i]);
+    load_words<NB>(vp, t.v[i]);
+    load_words<2 * NB>(sp, t.ks[i]);
+    load_words<2 * NB>(sp + 8 * NB, t.vs[i]);
+  }
+}
+
+// The wave's state for its 16 columns.
+template <int NB, int P>
+struct Acc {
+  f32x4 o[2 * NB];  // O^T tiles, scaled like P
+  float ref, sum;   // M, and this lane's part of sum P
+};
+
+// Q^T as B operands, P parts per block.
+template <int NB, int P>
+struct Query {
+  f16x8 q[NB][P];
+  float fac;  // score from the product: scale * log2(e) / 2^k
+};
+
+template <typename T>
+__device__ inline void load8f(const T *p, float (&x)[8]);
+template <>
+__device__ inline void load8f<float>(const float *p, float (&x)[8]) {
+  const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+}
+template <>
+__device__ inline void load8f<f16>(const f16 *p, float (&x)[8]) {
+  const f16x8 a = *reinterpret_cast<const f16x8 *>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+}
+
+// q of the lane's column (the 8 elements of each block that slot group g
+// multiplies).  An f32 row is brought to [2^10, 2^11) by a power of two 2^k, so
+// that its low parts lose nothing that counts.
+template <int NB, int P, typename T>
+__device__ inline void load_query(Query<NB, P> &Q, const T *q, bool there, uint32_t g, float scale) {
+  float x[NB][8], top = 0;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    if (there) {
+      load8f<T>(q + 32 * b + 8 * g, x[b]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[b][e] = 0;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, __builtin_fabsf(x[b][e]));
+  }
+  int k = 0;
+  if (P == 2) {
+    top = max_across(top);
+    k = top > 0 && top < __builtin_inff() ? 11 - __builtin_amdgcn_frexp_expf(top) : 0;
+    k = k < -100 ? -100 : k > 100 ? 100 : k;
+  }
+  Q.fac = __builtin_ldexpf(__builtin_fabsf(scale) * 1.4426950408889634f, -k);
+  const float sign = scale < 0 ? -1.0f : 1.0f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      f16x8 h;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (p == 0) x[b][e] = __builtin_ldexpf(x[b][e], k) * sign;
+        h[e] = (f16)x[b][e];
+        x[b][e] -= (float)h[e];
+      }
+      Q.q[b][p] = h;
+    }
+}
+
+// Nibbles 0 and 4 (HIGH: 1 and 5) of w as the codes' values: the f16 numbers
+// 1024 + n (64 + n for the high ones, four bits further up), less 1024 (64) and
+// the codes' 8.  Exact.
+template <bool HIGH>
+__device__ inline f16x2 codes(uint32_t w) {
+  const f16 off = HIGH ? (f16)-72.0f : (f16)-1032.0f;
+  return as_f16x2(HIGH ? (w & 0x00f000f0u) | 0x54005400u : (w & 0x000f000fu) | 0x64006400u) + (f16x2){off, off};
+}
+
+// One step.  `bound` is whether any column misses some of the keys; then lane
+// column's keys are [lo, hi) and pages may be missing.
+template <int NB, int P>
+__device__ inline void step(Acc<NB, P> &A, const Query<NB, P> &Q, const Step<NB> &t, bool bound, int32_t key,
+                            int32_t lo, int32_t hi, int32_t len, uint32_t g) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float s[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const uint32_t w = t.k[i][b], y = w >> 8;
+      const f16x8 kk = as_f16x8(as_u32(codes<false>(w)), as_u32(codes<true>(w)), as_u32(codes<false>(y)),
+                                as_u32(codes<true>(y)));
+      f32x4 d = {0, 0, 0, 0};
+#pragma unroll
+      for (int p = 0; p < P; ++p) d = mfma(kk, Q.q[b][p], d);
+      const f16x2 s01 = as_f16x2(t.ks[i][2 * b]), s23 = as_f16x2(t.ks[i][2 * b + 1]);
+      s[0] = __builtin_fmaf((float)s01.x, d[0], s[0]);
+      s[1] = __builtin_fmaf((float)s01.y, d[1], s[1]);
+      s[2] = __builtin_fmaf((float)s23.x, d[2], s[2]);
+      s[3] = __builtin_fmaf((float)s23.y, d[3], s[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 * i + j] = s[j] * Q.fac;
+  }
+  uint32_t seen = 0xff;
+  if (bound) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int32_t j = key + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
+      const bool ok = j >= lo && j < hi && t.there[i / 4];
+      if (!ok) {
+        x[i] = -__builtin_inff();
+        seen &= ~(1u << i);
+      }
+    }
+  }
+  float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3])),
+                              __builtin_fmaxf(__builtin_fmaxf(x[4], x[5]), __builtin_fmaxf(x[6], x[7])));
+  if (__any(top > A.ref + kRaise)) {
+    top = max_across(top);
+    // the reference of a column that has seen no key stays
+    const float ref = top > A.ref + kRaise ? top - kLift : A.ref;
+    const float f = __builtin_amdgcn_exp2f(A.ref - ref);
+    A.ref = ref;
+    A.sum *= f;
+#pragma unroll
+    for (int n = 0; n < 2 * NB; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) A.o[n][j] *= f;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = __builtin_amdgcn_exp2f(x[i] - A.ref);
+    if (bound && !(seen >> i & 1)) x[i] = 0;
+    A.sum += x[i];
+  }
+  f16x8 pr[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      pr[p][i] = (f16)x[i];
+      x[i] -= (float)pr[p][i];
+    }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    f16x2 s[4] = {as_f16x2(t.vs[0][2 * b]), as_f16x2(t.vs[0][2 * b + 1]), as_f16x2(t.vs[1][2 * b]),
+                  as_f16x2(t.vs[1][2 * b + 1])};
+    if (bound) {
+      // What lies past the end or on a page that is not there may be any bits:
+      // with a scale of 0 it stands for 0.
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int32_t j = key + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
+        if (!(j < len && t.there[i / 4])) s[i / 2][i % 2] = (f16)0.0f;
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      // lanes' words hold tokens 0 2 1 3: (tok0, tok1) then (tok2, tok3)
+      uint32_t hi2[4], lo2[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t w = t.v[i][b] >> (8 * j);
+          const f16x2 n = half ? codes<true>(w) : codes<false>(w);
+          const f16x2 v = n * s[2 * i + j];
+          hi2[2 * i + j] = as_u32(v);
+          if (P == 2) lo2[2 * i + j] = as_u32(__builtin_elementwise_fma(n, s[2 * i + j], -v));
+        }
+      f32x4 d = A.o[2 * b + half];
+      const f16x8 vh = as_f16x8(hi2[0], hi2[1], hi2[2], hi2[3]);
+      if (P == 2) {
+        const f16x8 vl = as_f16x8(lo2[0], lo2[1], lo2[2], lo2[3]);
+        d = mfma(vl, pr[0], d);
+        d = mfma(vh, pr[P - 1], d);
+      }
+      A.o[2 * b + half] = mfma(vh, pr[0], d);
+    }
+  }
+}
+
+// The 32-key steps [first, first + steps) that some column of the tile sees,
+// and the split of them over workgroups: `per` steps each, `active` shares.
+struct Range {
+  int32_t first, steps, per, active;
+};
+__device__ inline Range key_range(const AttnArgs &a, const Kv4Seq &s, uint32_t col0, uint32_t cols) {
+  Range r;
+  int32_t lo = 0, hi = s.len;
+  if (a.causal) {
+    const uint32_t last = (col0 + kCols < cols ? col0 + kCols : cols) - 1;
+    const int32_t p0 = s.pos0 + (int32_t)(col0 / a.group), p1 = s.pos0 + (int32_t)(last / a.group);
+    hi = p1 + 1 < hi ? p1 + 1 : hi;
+    if (a.window && p0 >= (int32_t)a.window) lo = p0 - (int32_t)a.window + 1;
+  }
+  hi = hi > 0 ? hi : 0;
+  r.first = lo / kKeys;
+  r.steps = (hi + kKeys - 1) / kKeys - r.first;
+  r.steps = r.steps > 0 ? r.steps : 0;
+  const int32_t even = (r.steps + (int32_t)a.splits - 1) / (int32_t)a.splits;
+  r.per = even > (int32_t)a.min_steps ? even : (int32_t)a.min_steps;
+  r.active = r.steps ? (r.steps + r.per - 1) / r.per : 1;
+  return r;
+}
+
+template <typename T>
+__device__ inline void put(T *out, float v);
+template <>
+__device__ inline void put<float>(float *out, float v) { *out = v; }
+template <>
+__device__ inline void put<f16>(f16 *out, float v) { *out = (f16)v; }
+
+// Workgroup: W waves on the same 16 columns, wave w taking steps w, w + W, ..
+// of the workgroup's share; their results meet in LDS.  Grid: tiles of columns x
+// splits, kv heads, sequences.
+template <int NB, int W, typename T>
+__global__ __launch_bounds__(64 * W) void kv4_attn_kernel(AttnArgs a) {
+  constexpr int P = sizeof(T) == 4 ? 2 : 1;
+  constexpr int D = NB * 32;
+  const uint32_t tile = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const uint32_t head = blockIdx.y, seq = blockIdx.z;
+  const Kv4Seq s = kv4_seq(a.kv, seq);
+  const uint32_t cols = s.nrows * a.group, col0 = tile * kCols;
+  if (col0 >= cols) return;
+  const Range rg = key_range(a, s, col0, cols);
+  if ((int32_t)split >= rg.active) return;
+
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t r = lane & 15, g = lane >> 4, col = col0 + r;
+  const bool mine = col < cols;
+  const uint32_t row = mine ? col / a.group : 0, sub = mine ? col % a.group : 0;
+  Query<NB, P> Q;
+  load_query<NB, P, T>(Q, static_cast<const T *>(a.q) + (size_t)(s.row0 + row) * a.ldq +
+                              (size_t)(head * a.group + sub) * D, mine, g, a.scale);
+  // keys the lane's column sees
+  int32_t lo = 0, hi = s.len;
+  if (a.causal) {
+    const int32_t p = s.pos0 + (int32_t)row;
+    hi = p + 1 < hi ? p + 1 : hi;
+    if (a.window && p >= (int32_t)a.window) lo = p - (int32_t)a.window + 1;
+  }
+  if (!mine) hi = 0;
+  // keys every column of the wave sees
+  int32_t all_lo = 0, all_hi = s.len;
+  if (a.causal) {
+    const uint32_t last = (col0 + kCols < cols ? col0 + kCols : cols) - 1;
+    const int32_t p0 = s.pos0 + (int32_t)(col0 / a.group), p1 = s.pos0 + (int32_t)(last / a.group);
+    all_hi = p0 + 1 < all_hi ? p0 + 1 : all_hi;
+    if (a.window && p1 >= (int32_t)a.window) all_lo = p1 - (int32_t)a.window + 1;
+  }
+
+  Acc<NB, P> A;
+  A.ref = kNever;
+  A.sum = 0;
+#pragma unroll
+  for (int n = 0; n < 2 * NB; ++n) A.o[n] = (f32x4){0, 0, 0, 0};
+
+  const int32_t end = rg.first + (((int32_t)split + 1) * rg.per < rg.steps ? ((int32_t)split + 1) * rg.per : rg.steps);
+  int32_t at = rg.first + (int32_t)split * rg.per + (int32_t)wave;
+  Step<NB> cur, nxt;
+  if (at < end) fetch<NB>(cur, a.kv, seq, head, at * kKeys, s.len, lane);
+  while (at < end) {
+    const int32_t next = at + W;
+    if (next < end) fetch<NB>(nxt, a.kv, seq, head, next * kKeys, s.len, lane);
+    const int32_t key = at * kKeys;
+    const bool bound = key < all_lo || key + kKeys > all_hi || !cur.there[0] || !cur.there[1];
+    step<NB, P>(A, Q, cur, bound, key, lo, hi, s.len, g);
+    cur = nxt;
+    at = next;
+  }
+  A.sum = sum_across(A.sum);
+
+  // the waves' results: a common reference, then sums over the waves
+  __shared__ float sh_ref[W][kCols], sh_sum[W][kCols];
+  __shared__ float sh_o[W][kCols][D + 4];
+  if (g == 0) {
+    sh_ref[wave][r] = A.ref;
+    sh_sum[wave][r] = A.sum;
+  }
+#pragma unroll
+  for (int n = 0; n < 2 * NB; ++n) *reinterpret_cast<f32x4 *>(&sh_o[wave][r][16 * n + 4 * g]) = A.o[n];
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < kCols * D; i += 64 * W) {
+    const uint32_t c = i / D, d = i % D;
+    if (col0 + c >= cols) break;
+    float ref = kNever, o = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) ref = __builtin_fmaxf(ref, sh_ref[w][c]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sh_ref[w][c] - ref);
+      sum = __builtin_fmaf(sh_sum[w][c], f, sum);
+      o = __builtin_fmaf(sh_o[w][c][d], f, o);
+    }
+    if (rg.active == 1) {
+      const uint32_t orow = s.row0 + (col0 + c) / a.group, oh = head * a.group + (col0 + c) % a.group;
+      put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + d, sum == 0 ? 0.0f : o / sum);
+    } else {
+      const uint32_t tiles = gridDim.x / a.splits;
+      float *w = a.work + ((((size_t)seq * gridDim.y + head) * tiles + tile) * a.splits + split) *
+                              (kCols * (D + 2));
+      w[i] = o;
+      if (d == 0) {
+        w[kCols * D + c] = ref;
+        w[kCols * D + kCols + c] = sum;
+      }
+    }
+  }
+}
+
+// The splits' results of one tile of columns, joined.  A workgroup per tile,
+// kv head and sequence.
+template <int NB, typename T>
+__global__ __launch_bounds__(256) void kv4_attn_join_kernel(AttnArgs a) {
+  constexpr int D = NB * 32;
+  const uint32_t tile = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
+  const Kv4Seq s = kv4_seq(a.kv, seq);
+  const uint32_t cols = s.nrows * a.group, col0 = tile * kCols;
+  if (col0 >= cols) return;
+  const Range rg = key_range(a, s, col0, cols);
+  if (rg.active == 1) return;
+  const float *w = a.work + (((size_t)seq * gridDim.y + head) * gridDim.x + tile) * a.splits * (kCols * (D + 2));
+  for (uint32_t i = threadIdx.x; i < kCols * D; i += 256) {
+    const uint32_t c = i / D, d = i % D;
+    if (col0 + c >= cols) break;
+    float ref = kNever, o = 0, sum = 0;
+    for (int32_t n = 0; n < rg.active; ++n)
+      ref = __builtin_fmaxf(ref, w[(size_t)n * (kCols * (D + 2)) + kCols * D + c]);
+    for (int32_t n = 0; n < rg.active; ++n) {
+      const float *p = w + (size_t)n * (kCols * (D + 2));
+      const float f = __builtin_amdgcn_exp2f(p[kCols * D + c] - ref);
+      sum = __builtin_fmaf(p[kCols * D + kCols + c], f, sum);
+      o = __builtin_fmaf(p[i], f, o);
+    }
+    const uint32_t orow = s.row0 + (col0 + c) / a.group, oh = head * a.group + (col0 + c) % a.group;
+    put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + d, sum == 0 ? 0.0f : o / sum);
+  }
+}
+
+struct Plan {
+  uint32_t tiles, splits, min_steps;
+  size_t share;  // bytes of one split of one tile
+};
+// How many workgroups share the keys of a tile: enough for two workgroups per
+// CU, none with less than eight steps (a step per wave twice).
+Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, uint32_t cus) {
+  Plan p;
+  const uint64_t reach = (uint64_t)b->max_pages * c->page;
+  const uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
+  const uint64_t cols = (uint64_t)b->rows * (nh / c->nkv);
+  p.tiles = (uint32_t)((cols + kCols - 1) / kCols);
+  p.min_steps = 8;
+  p.share = (size_t)kCols * (c->d + 2) * 4;
+  const uint64_t groups = (uint64_t)p.tiles * c->nkv * b->b, steps = (len + kKeys - 1) / kKeys;
+  uint64_t want = groups ? (2ull * cus + groups - 1) / groups : 1;
+  const uint64_t most = steps / p.min_steps;
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  if (want > 256) want = 256;
+  p.splits = (uint32_t)want;
+  return p;
+}
+
+template <int NB, typename T>
+void launch(const AttnArgs &a, uint32_t tiles, uint32_t b) {
+  kv4_attn_kernel<NB, 4, T><<<dim3(tiles * a.splits, a.kv.nkv, b), 256, 0, stream()>>>(a);
+  if (a.splits > 1) kv4_attn_join_kernel<NB, T><<<dim3(tiles, a.kv.nkv, b), 256, 0, stream()>>>(a);
+}
+
+}  // namespace
+
+extern "C" size_t madi_kv4_attn_bytes(const madi_kv4 *cache, const madi_kv4_batch *batch, uint32_t nh) {
+  Kv4Args a;
+  if (kv4_args("madi_kv4_attn_bytes", cache, batch, &a) || nh == 0 || nh % cache->nkv) return 0;
+  const Plan p = plan_of(cache, batch, nh, initialized() ? (uint32_t)cu_count() : 256);
+  return p.splits > 1 ? (size_t)p.tiles * cache->nkv * batch->b * p.splits * p.share : 0;
+}
+
+extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, const madi_kv4_batch *batch,
+                             uint32_t nh, uint32_t ldo, uint32_t ldq, uint32_t window, int causal, int dtype,
+                             float scale) {
+  const char *what = "madi_kv4_attn";
+  AttnArgs a;
+  if (int rc = kv4_args(what, cache, batch, &a.kv)) return rc;
+  if (nh == 0 || nh % cache->nkv)
+    return fail(MADI_ERR_SHAPE, "%s: %u query heads over %u kv heads", what, nh, cache->nkv);
+  const uint64_t width = (uint64_t)nh * cache->d;
+  size_t qb, ob;
+  if (int rc = kv4_rows(what, "q", q, batch->m, width, ldq, dtype, &qb)) return rc;
+  if (int rc = kv4_rows(what, "out", out, batch->m, width, ldo, dtype, &ob)) return rc;
+  if (causal != 0 && causal != 1) return fail(MADI_ERR_ARG, "%s: causal %d", what, causal);
+  if (!causal && window) return fail(MADI_ERR_ARG, "%s: a window without causal", what);
+  if (window > 0x7fffffffu) window = 0;  // wider than any cache
+  if (!(__builtin_fabsf(scale) < __builtin_inff())) return fail(MADI_ERR_ARG, "%s: scale %g", what, scale);
+  if (batch->work && !aligned(batch->work, 16)) return fail(MADI_ERR_ALIGN, "%s: work must be 16-byte aligned", what);
+  const size_t cb = kv4_cache_bytes(cache), wb = batch->work ? batch->work_bytes : 0;
+  if (kv4_overlap(out, ob, cache->data, cb) || (kv4_overlap(out, ob, q, qb) && !(out == q && ldo == ldq)) ||
+      kv4_overlap(out, ob, batch->work, wb) || kv4_overlap(q, qb, batch->work, wb) ||
+      kv4_overlap(cache->data, cb, batch->work, wb))
+    return fail(MADI_ERR_ARG, "%s: out or work overlaps another operand", what);
+  if ((uint64_t)batch->rows * (nh / cache->nkv) > 0x7fffffffu)
+    return fail(MADI_ERR_SHAPE, "%s: %u rows of a sequence in one call", what, batch->rows);
+  if (!initialized()) return fail(MADI_ERR_NOT_INIT, "%s: madi_init has not succeeded", what);
+  if (batch->m == 0 || batch->b == 0 || batch->rows == 0) return MADI_OK;
+  Plan p = plan_of(cache, batch, nh, (uint32_t)cu_count());
+  // as many splits as the workspace holds
+  const size_t each = (size_t)p.tiles * cache->nkv * batch->b * p.share;
+  if ((size_t)p.splits * each > wb) p.splits = wb / each > 1 ? (uint32_t)(wb / each) : 1;
+  if ((uint64_t)p.tiles * p.splits > 0x7fffffffu)
+    return fail(MADI_ERR_SHAPE, "%s: %u rows of a sequence in one call", what, batch->rows);
+  if (int rc = deferred_before_read(q, qb)) return rc;
+  if (int rc = deferred_before_read(cache->data, cb)) return rc;
+  if (int rc = deferred_before_write(out, ob)) return rc;
+  if (p.splits > 1)
+    if (int rc = deferred_before_write(batch->work, wb)) return rc;
+  a.q = q;
+  a.out = out;
+  a.work = static_cast<float *>(batch->work);
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.group = nh / cache->nkv;
+  a.window = window;
+  a.causal = (uint32_t)causal;
+  a.splits = p.splits;
+  a.min_steps = p.min_steps;
+  a.scale = scale;
+  const bool f = dtype == MADI_F32;
+  switch (cache->d) {
+  case 64: f ? launch<2, float>(a, p.tiles, batch->b) : launch<2, f16>(a, p.tiles, batch->b); break;
+  case 96: f ? launch<3, float>(a, p.tiles, batch->b) : launch<3, f16>(a, p.tiles, batch->b); break;
+  case 128: f ? launch<4, float>(a, p.tiles, batch->b) : launch<4, f16>(a, p.tiles, batch->b); break;
+  default: f ? launch<8, float>(a, p.tiles, batch->b) : launch<8, f16>(a, p.tiles, batch->b); break;
+  }
+  return check_launch(what);
+}

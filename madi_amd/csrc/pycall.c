@@ -56,6 +56,8 @@ typedef uintptr_t u;
 #define F(...) ((int (*)(__VA_ARGS__))addr)
 static int invoke(uintptr_t addr, int ni, int nf, const uint64_t *a, const float *f) {
   if (nf == 2 && ni == 6) return F(u, u, u, u, u, u, float, float)(a[0], a[1], a[2], a[3], a[4], a[5], f[0], f[1]);
+  if (nf == 1 && ni == 10)
+    return F(u, u, u, u, u, u, u, u, u, u, float)(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], f[0]);
   switch (ni) {
   case 0: return F(void)();
   case 1: return F(u)(a[0]);
@@ -140,7 +142,7 @@ static PyObject *bind(PyObject *mod, PyObject *args) {
     else if (*s == 'p' || *s == 'i') ++ni;
     else return PyErr_Format(PyExc_ValueError, "signature letter '%c'", *s);
   }
-  if (ni > MAX_INTS || (nf != 0 && !(nf == 2 && ni == 6)))
+  if (ni > MAX_INTS || (nf != 0 && !(nf == 2 && ni == 6) && !(nf == 1 && ni == 10)))
     return PyErr_Format(PyExc_ValueError, "signature '%s' has no call form", sig);
   Call *c = PyObject_New(Call, &CallType);
   if (!c) return NULL;
