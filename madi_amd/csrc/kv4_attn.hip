@@ -13,9 +13,11 @@
 //     it by 2^8, so most steps exchange nothing between lanes.
 //   O^T += V^T P^T, 32 keys as K and 16 elements as rows: P^T comes straight
 //     from the S^T registers (lane (g, c) holds keys 4g..4g+3 of both tiles),
-//     V as (n - 8) s in f16 from the words that hold four tokens.
-// f32 rows: q, P and V are each split in two f16 (22 bits; V's 15 bits exactly),
-// the products with both low parts left out (2^-22).
+//     V as (n - 8) s in f16 from the words that hold four tokens.  P goes in as
+//     two f16 (22 bits): with one, its rounding beside V's took f16 results from
+//     1.2 to 1.6 of the error that rounding the exact result to f16 has.
+// f32 rows: q and V too are split in two f16 (22 bits; V's 15 bits exactly), the
+// product of both low parts left out (2^-22).
 #include "kv4.h"
 
 using namespace madi;
@@ -38,6 +40,8 @@ struct AttnArgs {
   uint32_t ldq, ldo, group, window, causal, splits, min_steps;
   float scale;
 };
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <int N>
 __device__ inline void load_words(const uint8_t *p, uint32_t (&w)[N]) {
@@ -86,24 +90,27 @@ struct Step {
   bool there[2];
 };
 
+// Pages of the tiles at key and key + 16 (none past the end).
+__device__ inline void find_pages(uint32_t (&page)[2], const Kv4Args &a, uint32_t seq, int32_t key, int32_t len) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) page[i] = key + 16 * i < len ? kv4_page(a, seq, key + 16 * i) : 0xffffffffu;
+}
+
 template <int NB>
-__device__ inline void fetch(Step<NB> &t, const Kv4Args &a, uint32_t seq, uint32_t head, int32_t key,
-                             int32_t len, uint32_t lane) {
+__device__ inline void fetch(Step<NB> &t, const Kv4Args &a, const uint32_t (&pages)[2], uint32_t head, int32_t key,
+                             uint32_t lane) {
   constexpr uint32_t D = NB * 32;
   const uint32_t r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    // a tile past the end has no page entry to read: any valid one stands in
-    const int32_t at = key + 16 * i;
-    uint32_t page = 0xffffffffu;
-    if (at < len) page = kv4_page(a, seq, at);
-    t.there[i] = page < a.n_pages;
-    if (!t.there[i]) page = 0;
-    const uint32_t off = (uint32_t)at & ((1u << a.shift) - 1);
+    // a tile without a page: any valid one stands in
+    t.there[i] = pages[i] < a.n_pages;
+    const uint32_t page = t.there[i] ? pages[i] : 0;
+    const uint32_t off = (uint32_t)(key + 16 * i) & ((1u << a.shift) - 1);
     const uint8_t *blk = kv4_block(a, page, head, D);
-    const uint8_t *kp = blk + (size_t)(off + r) * (D / 2) + g * (4 * NB);
-    const uint8_t *vp = blk + ((size_t)(D / 2) << a.shift) + (size_t)(off / 4 + g) * (2 * D) + r * (4 * NB);
-    const uint8_t *sp = blk + ((size_t)D << a.shift) + (size_t)(off / 4 + g) * (D / 2);
+    const uint8_t *kp = blk + (size_t)off * (D / 2) + (r * (D / 2) + g * (4 * NB));
+    const uint8_t *vp = blk + ((size_t)(D / 2) << a.shift) + (size_t)(off / 4) * (2 * D) + (g * (2 * D) + r * (4 * NB));
+    const uint8_t *sp = blk + ((size_t)D << a.shift) + (size_t)(off / 4) * (D / 2) + g * (D / 2);
     load_words<NB>(kp, t.k[i]);
     load_words<NB>(vp, t.v[i]);
     load_words<2 * NB>(sp, t.ks[i]);
@@ -112,7 +119,7 @@ __device__ inline void fetch(Step<NB> &t, const Kv4Args &a, uint32_t seq, uint32
 }
 
 // The wave's state for its 16 columns.
-template <int NB, int P>
+template <int NB>
 struct Acc {
   f32x4 o[2 * NB];  // O^T tiles, scaled like P
   float ref, sum;   // M, and this lane's part of sum P
@@ -163,7 +170,8 @@ __device__ inline void load_query(Query<NB, P> &Q, const T *q, bool there, uint3
     k = top > 0 && top < __builtin_inff() ? 11 - __builtin_amdgcn_frexp_expf(top) : 0;
     k = k < -100 ? -100 : k > 100 ? 100 : k;
   }
-  Q.fac = __builtin_ldexpf(__builtin_fabsf(scale) * 1.4426950408889634f, -k);
+  // (never 0, so that it leaves the - infinity of a key not seen what it is)
+  Q.fac = __builtin_fmaxf(__builtin_ldexpf(__builtin_fabsf(scale) * 1.4426950408889634f, -k), 1e-37f);
   const float sign = scale < 0 ? -1.0f : 1.0f;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -182,53 +190,77 @@ __device__ inline void load_query(Query<NB, P> &Q, const T *q, bool there, uint3
 
 // Nibbles 0 and 4 (HIGH: 1 and 5) of w as the codes' values: the f16 numbers
 // 1024 + n (64 + n for the high ones, four bits further up), less 1024 (64) and
-// the codes' 8.  Exact.
+// the codes' 8.  Exact.  The masks are in VGPRs: an instruction reads one SGPR or
+// literal, and v_and_or_b32 wants two constants.
+struct Masks {
+  uint32_t lo, hi;
+  float minus1;
+};
+__device__ inline Masks masks() {
+  Masks m = {0x000f000fu, 0x00f000f0u, -1.0f};
+  asm("" : "+v"(m.lo), "+v"(m.hi), "+v"(m.minus1));
+  return m;
+}
 template <bool HIGH>
-__device__ inline f16x2 codes(uint32_t w) {
+__device__ inline f16x2 codes(const Masks &m, uint32_t w) {
   const f16 off = HIGH ? (f16)-72.0f : (f16)-1032.0f;
-  return as_f16x2(HIGH ? (w & 0x00f000f0u) | 0x54005400u : (w & 0x000f000fu) | 0x64006400u) + (f16x2){off, off};
+  return as_f16x2(HIGH ? (w & m.hi) | 0x54005400u : (w & m.lo) | 0x64006400u) + (f16x2){off, off};
 }
 
-// One step.  `bound` is whether any column misses some of the keys; then lane
-// column's keys are [lo, hi) and pages may be missing.
+// Scores of a step, without the factor: x[4i + j] is key 16i + 4g + j.
 template <int NB, int P>
-__device__ inline void step(Acc<NB, P> &A, const Query<NB, P> &Q, const Step<NB> &t, bool bound, int32_t key,
-                            int32_t lo, int32_t hi, int32_t len, uint32_t g) {
-  float x[8];
+__device__ inline void scores(float (&x)[8], const Query<NB, P> &Q, const Step<NB> &t, const Masks &m) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    float s[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const uint32_t w = t.k[i][b], y = w >> 8;
-      const f16x8 kk = as_f16x8(as_u32(codes<false>(w)), as_u32(codes<true>(w)), as_u32(codes<false>(y)),
-                                as_u32(codes<true>(y)));
+      const f16x8 kk = as_f16x8(as_u32(codes<false>(m, w)), as_u32(codes<true>(m, w)), as_u32(codes<false>(m, y)),
+                                as_u32(codes<true>(m, y)));
       f32x4 d = {0, 0, 0, 0};
 #pragma unroll
       for (int p = 0; p < P; ++p) d = mfma(kk, Q.q[b][p], d);
       const f16x2 s01 = as_f16x2(t.ks[i][2 * b]), s23 = as_f16x2(t.ks[i][2 * b + 1]);
-      s[0] = __builtin_fmaf((float)s01.x, d[0], s[0]);
-      s[1] = __builtin_fmaf((float)s01.y, d[1], s[1]);
-      s[2] = __builtin_fmaf((float)s23.x, d[2], s[2]);
-      s[3] = __builtin_fmaf((float)s23.y, d[3], s[3]);
+      const f16 s[4] = {s01.x, s01.y, s23.x, s23.y};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = __builtin_fmaf((float)s[j], d[j], b ? x[4 * i + j] : 0.0f);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[4 * i + j] = s[j] * Q.fac;
   }
-  uint32_t seen = 0xff;
-  if (bound) {
+}
+
+// A step that some column does not see all of: the lane's column sees [lo, hi),
+// and none of a tile whose page is not there.  What lies past the end or
+// stands in for such a page may be any bits: with a V scale of 0 it is 0.
+template <int NB>
+__device__ inline void cut(float (&x)[8], Step<NB> &t, int32_t key, int32_t lo, int32_t hi, int32_t len, uint32_t g) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int32_t j = key + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
-      const bool ok = j >= lo && j < hi && t.there[i / 4];
-      if (!ok) {
-        x[i] = -__builtin_inff();
-        seen &= ~(1u << i);
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int32_t k = key + 16 * i + 4 * (int32_t)g + j;
+      if (!(k >= lo && k < hi && t.there[i])) x[4 * i + j] = -__builtin_inff();
+      if (!(k < len && t.there[i])) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) t.vs[i][2 * b + j / 2] &= j % 2 ? 0x0000ffffu : 0xffff0000u;
       }
     }
-  }
+}
+
+// Two f32 as f16 pairs: their roundings and what those leave (exact), rounded.
+// (minus1: -1 in a register, which keeps x - hi one instruction that takes hi as f16.)
+__device__ inline void split_pair(float minus1, float x, float y, uint32_t &hi, uint32_t &lo) {
+  const f16x2 h = __builtin_convertvector(((f32x2){x, y}), f16x2);
+  const f32x2 r = {__builtin_fmaf((float)h.x, minus1, x), __builtin_fmaf((float)h.y, minus1, y)};
+  hi = as_u32(h);
+  lo = as_u32(__builtin_convertvector(r, f16x2));
+}
+
+// Softmax weights of a step and their product with V.
+template <int NB, int P>
+__device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const Step<NB> &t, const Masks &m) {
   float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3])),
                               __builtin_fmaxf(__builtin_fmaxf(x[4], x[5]), __builtin_fmaxf(x[6], x[7])));
+  top *= fac;
   if (__any(top > A.ref + kRaise)) {
     top = max_across(top);
     // the reference of a column that has seen no key stays
@@ -241,57 +273,38 @@ __device__ inline void step(Acc<NB, P> &A, const Query<NB, P> &Q, const Step<NB>
 #pragma unroll
       for (int j = 0; j < 4; ++j) A.o[n][j] *= f;
   }
+  uint32_t hi[4], lo[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = __builtin_amdgcn_exp2f(x[i] - A.ref);
-    if (bound && !(seen >> i & 1)) x[i] = 0;
-    A.sum += x[i];
+  for (int i = 0; i < 4; ++i) {
+    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], fac, -A.ref));
+    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], fac, -A.ref));
+    A.sum += x0;
+    A.sum += x1;
+    split_pair(m.minus1, x0, x1, hi[i], lo[i]);
   }
-  f16x8 pr[P];
+  const f16x8 ph = as_f16x8(hi[0], hi[1], hi[2], hi[3]), pl = as_f16x8(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
-  for (int p = 0; p < P; ++p)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      pr[p][i] = (f16)x[i];
-      x[i] -= (float)pr[p][i];
-    }
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    f16x2 s[4] = {as_f16x2(t.vs[0][2 * b]), as_f16x2(t.vs[0][2 * b + 1]), as_f16x2(t.vs[1][2 * b]),
-                  as_f16x2(t.vs[1][2 * b + 1])};
-    if (bound) {
-      // What lies past the end or on a page that is not there may be any bits:
-      // with a scale of 0 it stands for 0.
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int32_t j = key + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
-        if (!(j < len && t.there[i / 4])) s[i / 2][i % 2] = (f16)0.0f;
-      }
-    }
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      // lanes' words hold tokens 0 2 1 3: (tok0, tok1) then (tok2, tok3)
-      uint32_t hi2[4], lo2[4];
+      // words hold tokens 0 2 1 3: (tok0, tok1) then (tok2, tok3)
+      uint32_t vh[4], vl[4];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t w = t.v[i][b] >> (8 * j);
-          const f16x2 n = half ? codes<true>(w) : codes<false>(w);
-          const f16x2 v = n * s[2 * i + j];
-          hi2[2 * i + j] = as_u32(v);
-          if (P == 2) lo2[2 * i + j] = as_u32(__builtin_elementwise_fma(n, s[2 * i + j], -v));
+          const f16x2 n = half ? codes<true>(m, w) : codes<false>(m, w), s = as_f16x2(t.vs[i][2 * b + j]);
+          const f16x2 v = n * s;
+          vh[2 * i + j] = as_u32(v);
+          if (P == 2) vl[2 * i + j] = as_u32(__builtin_elementwise_fma(n, s, -v));
         }
       f32x4 d = A.o[2 * b + half];
-      const f16x8 vh = as_f16x8(hi2[0], hi2[1], hi2[2], hi2[3]);
-      if (P == 2) {
-        const f16x8 vl = as_f16x8(lo2[0], lo2[1], lo2[2], lo2[3]);
-        d = mfma(vl, pr[0], d);
-        d = mfma(vh, pr[P - 1], d);
-      }
-      A.o[2 * b + half] = mfma(vh, pr[0], d);
+      const f16x8 v8 = as_f16x8(vh[0], vh[1], vh[2], vh[3]);
+      d = mfma(v8, pl, d);
+      if (P == 2) d = mfma(as_f16x8(vl[0], vl[1], vl[2], vl[3]), ph, d);
+      A.o[2 * b + half] = mfma(v8, ph, d);
     }
-  }
 }
 
 // The 32-key steps [first, first + steps) that some column of the tile sees,
@@ -329,7 +342,7 @@ __device__ inline void put<f16>(f16 *out, float v) { *out = (f16)v; }
 // of the workgroup's share; their results meet in LDS.  Grid: tiles of columns x
 // splits, kv heads, sequences.
 template <int NB, int W, typename T>
-__global__ __launch_bounds__(64 * W) void kv4_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * W, NB == 8 ? 1 : 2) void kv4_attn_kernel(AttnArgs a) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
   constexpr int D = NB * 32;
   const uint32_t tile = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
@@ -340,7 +353,7 @@ __global__ __launch_bounds__(64 * W) void kv4_attn_kernel(AttnArgs a) {
   const Range rg = key_range(a, s, col0, cols);
   if ((int32_t)split >= rg.active) return;
 
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t r = lane & 15, g = lane >> 4, col = col0 + r;
   const bool mine = col < cols;
   const uint32_t row = mine ? col / a.group : 0, sub = mine ? col % a.group : 0;
@@ -364,7 +377,7 @@ __global__ __launch_bounds__(64 * W) void kv4_attn_kernel(AttnArgs a) {
     if (a.window && p1 >= (int32_t)a.window) all_lo = p1 - (int32_t)a.window + 1;
   }
 
-  Acc<NB, P> A;
+  Acc<NB> A;
   A.ref = kNever;
   A.sum = 0;
 #pragma unroll
@@ -372,16 +385,28 @@ __global__ __launch_bounds__(64 * W) void kv4_attn_kernel(AttnArgs a) {
 
   const int32_t end = rg.first + (((int32_t)split + 1) * rg.per < rg.steps ? ((int32_t)split + 1) * rg.per : rg.steps);
   int32_t at = rg.first + (int32_t)split * rg.per + (int32_t)wave;
-  Step<NB> cur, nxt;
-  if (at < end) fetch<NB>(cur, a.kv, seq, head, at * kKeys, s.len, lane);
+  // Two steps' words in registers, one used while the other arrives, and the
+  // page numbers one step further ahead.
+  Step<NB> st[2];
+  uint32_t pages[2];
+  const Masks m = masks();
+  find_pages(pages, a.kv, seq, at * kKeys, at < end ? s.len : 0);
+  if (at < end) fetch<NB>(st[0], a.kv, pages, head, at * kKeys, lane);
+  find_pages(pages, a.kv, seq, (at + W) * kKeys, at + W < end ? s.len : 0);
   while (at < end) {
-    const int32_t next = at + W;
-    if (next < end) fetch<NB>(nxt, a.kv, seq, head, next * kKeys, s.len, lane);
-    const int32_t key = at * kKeys;
-    const bool bound = key < all_lo || key + kKeys > all_hi || !cur.there[0] || !cur.there[1];
-    step<NB, P>(A, Q, cur, bound, key, lo, hi, s.len, g);
-    cur = nxt;
-    at = next;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (at + W < end) fetch<NB>(st[1 - i], a.kv, pages, head, (at + W) * kKeys, lane);
+      find_pages(pages, a.kv, seq, (at + 2 * W) * kKeys, at + 2 * W < end ? s.len : 0);
+      const int32_t key = at * kKeys;
+      float x[8];
+      scores<NB, P>(x, Q, st[i], m);
+      if (key < all_lo || key + kKeys > all_hi || !st[i].there[0] || !st[i].there[1])
+        cut<NB>(x, st[i], key, lo, hi, s.len, g);
+      add_values<NB, P>(A, x, Q.fac, st[i], m);
+      at += W;
+      if (at >= end) break;
+    }
   }
   A.sum = sum_across(A.sum);
 
