@@ -13,11 +13,15 @@
 //     it by 2^8, so most steps exchange nothing between lanes.
 //   O^T += V^T P^T, 32 keys as K and 16 elements as rows: P^T comes straight
 //     from the S^T registers (lane (g, c) holds keys 4g..4g+3 of both tiles),
-//     V as (n - 8) s in f16 from the words that hold four tokens.  P goes in as
-//     two f16 (22 bits): with one, its rounding beside V's took f16 results from
-//     1.2 to 1.6 of the error that rounding the exact result to f16 has.
-// f32 rows: q and V too are split in two f16 (22 bits; V's 15 bits exactly), the
-// product of both low parts left out (2^-22).
+//     V as its codes from the words that hold four tokens, and the V scale of a
+//     key and block goes into P: one rounding, of P s, instead of P's and V's.
+//     s comes times 2^-e, e the largest exponent among the wave's V scales so
+//     far, so that P s stays within f16.
+// A lane holds two of the 8 nb scales of its four keys and passes them to the
+// other 15 through DPP broadcasts, which cost nothing in a multiplication.
+// f32 rows: q and P s are each split in two f16 (22 bits).
+#include <type_traits>
+
 #include "kv4.h"
 
 using namespace madi;
@@ -28,9 +32,14 @@ constexpr int kCols = 16;  // columns of a wave (MFMA columns)
 constexpr int kKeys = 32;  // keys of a step
 constexpr float kNever = -1e30f;  // reference before any key was seen
 // P is 2^(x - M) with M at first the largest x - 7, raised when an x passes M
-// by 15: P at most 2^15 (f16 holds 2^16), and a P that rounds to nothing is
-// 2^-32 of the largest.
-constexpr float kLift = 7.0f, kRaise = 15.0f;
+// by 14: P at most 2^14, P s 2^-e at most 2^15 (f16 holds 2^16), and what
+// rounds to nothing is 2^-32 of the largest P at the largest s.
+constexpr float kLift = 7.0f, kRaise = 14.0f;
+
+constexpr int kMaxSplits = 256;
+// f32 numbers of a share: O [16][D], then the references and the sums.
+template <int D>
+constexpr size_t kShare = kCols * (D + 2);
 
 struct AttnArgs {
   Kv4Args kv;
@@ -81,12 +90,33 @@ __device__ inline float max_across(float v) {
   swap32(__builtin_fmaxf(x, y), x, y);
   return __builtin_fmaxf(x, y);
 }
+// over the wave
+template <int CTRL>
+__device__ inline float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ inline float wave_sum(float v) {
+  v += dpp<0x121>(v);  // row_ror 1, 2, 4, 8
+  v += dpp<0x122>(v);
+  v += dpp<0x124>(v);
+  v += dpp<0x128>(v);
+  return sum_across(v);
+}
+__device__ inline float wave_max(float v) {
+  v = __builtin_fmaxf(v, dpp<0x121>(v));
+  v = __builtin_fmaxf(v, dpp<0x122>(v));
+  v = __builtin_fmaxf(v, dpp<0x124>(v));
+  v = __builtin_fmaxf(v, dpp<0x128>(v));
+  return max_across(v);
+}
 
 // One step's 32 keys as they lie in the cache, and whether their pages exist.
+// Scale i = x * 4 nb + 4 b + token (x 0 for K, 1 for V) of the four tokens of
+// group g is half i % 2 of word i / 2, which lane i / 2 % 16 of the group holds.
 template <int NB>
 struct Step {
-  uint32_t k[2][NB], v[2][NB];
-  uint32_t ks[2][2 * NB], vs[2][2 * NB];  // f16 [block][4 tokens]
+  static constexpr int kScaleWords = (NB + 3) / 4;
+  uint32_t k[2][NB], v[2][NB], s[2][kScaleWords];
   bool there[2];
 };
 
@@ -111,10 +141,14 @@ __device__ inline void fetch(Step<NB> &t, const Kv4Args &a, const uint32_t (&pag
     const uint8_t *kp = blk + (size_t)off * (D / 2) + (r * (D / 2) + g * (4 * NB));
     const uint8_t *vp = blk + ((size_t)(D / 2) << a.shift) + (size_t)(off / 4) * (2 * D) + (g * (2 * D) + r * (4 * NB));
     const uint8_t *sp = blk + ((size_t)D << a.shift) + (size_t)(off / 4) * (D / 2) + g * (D / 2);
+    constexpr uint32_t kWords = 4 * NB;  // of a group
     load_words<NB>(kp, t.k[i]);
     load_words<NB>(vp, t.v[i]);
-    load_words<2 * NB>(sp, t.ks[i]);
-    load_words<2 * NB>(sp + 8 * NB, t.vs[i]);
+#pragma unroll
+    for (uint32_t n = 0; n < Step<NB>::kScaleWords; ++n) {
+      const uint32_t w = 16 * n + r;  // (nb < 4: lanes past the words hold the last one)
+      load_words<1>(sp + 4 * (w < kWords ? w : kWords - 1), *reinterpret_cast<uint32_t(*)[1]>(&t.s[i][n]));
+    }
   }
 }
 
@@ -123,6 +157,7 @@ template <int NB>
 struct Acc {
   f32x4 o[2 * NB];  // O^T tiles, scaled like P
   float ref, sum;   // M, and this lane's part of sum P
+  float down, most; // 2^-e, and the largest V scale that it serves
 };
 
 // Q^T as B operands, P parts per block.
@@ -207,43 +242,70 @@ __device__ inline f16x2 codes(const Masks &m, uint32_t w) {
   return as_f16x2(HIGH ? (w & m.hi) | 0x54005400u : (w & m.lo) | 0x64006400u) + (f16x2){off, off};
 }
 
+// Lane LANE's word, or number, for each of its 16 (row_newbcast).
+template <int LANE>
+__device__ inline uint32_t word_from_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x150 + LANE, 0xf, 0xf, true);
+}
+template <int LANE>
+__device__ inline float from_lane(float v) {
+  return __builtin_bit_cast(float, word_from_lane<LANE>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int N, typename F>
+__device__ inline void each(F f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>());
+  }
+}
+
 // Scores of a step, without the factor: x[4i + j] is key 16i + 4g + j.
 template <int NB, int P>
 __device__ inline void scores(float (&x)[8], const Query<NB, P> &Q, const Step<NB> &t, const Masks &m) {
+  each<NB>([&](auto B) {
+    constexpr int b = B();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
+    for (int i = 0; i < 2; ++i) {
       const uint32_t w = t.k[i][b], y = w >> 8;
       const f16x8 kk = as_f16x8(as_u32(codes<false>(m, w)), as_u32(codes<true>(m, w)), as_u32(codes<false>(m, y)),
                                 as_u32(codes<true>(m, y)));
       f32x4 d = {0, 0, 0, 0};
 #pragma unroll
       for (int p = 0; p < P; ++p) d = mfma(kk, Q.q[b][p], d);
-      const f16x2 s01 = as_f16x2(t.ks[i][2 * b]), s23 = as_f16x2(t.ks[i][2 * b + 1]);
-      const f16 s[4] = {s01.x, s01.y, s23.x, s23.y};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * i + j] = __builtin_fmaf((float)s[j], d[j], b ? x[4 * i + j] : 0.0f);
+      // (as f16 pairs: a multiply-add takes a half of a word, but no DPP operand)
+      each<2>([&](auto J) {
+        constexpr int j = J(), word = 2 * b + j;
+        const f16x2 s = as_f16x2(word_from_lane<word % 16>(t.s[i][word / 16]));
+        x[4 * i + 2 * j] = __builtin_fmaf((float)s.x, d[2 * j], b ? x[4 * i + 2 * j] : 0.0f);
+        x[4 * i + 2 * j + 1] = __builtin_fmaf((float)s.y, d[2 * j + 1], b ? x[4 * i + 2 * j + 1] : 0.0f);
+      });
     }
-  }
+    if (b % 2) __builtin_amdgcn_sched_barrier(0);
+  });
 }
 
-// A step that some column does not see all of: the lane's column sees [lo, hi),
-// and none of a tile whose page is not there.  What lies past the end or
-// stands in for such a page may be any bits: with a V scale of 0 it is 0.
+// A step that some column does not see all of.  First the scales of what lies
+// past the end or stands in for a page that is not there become 0 (those bits may be
+// anything, and 0 times an infinity is not 0), then the scores of the keys that
+// the lane's column does not see, [lo, hi) it does, - infinity.
 template <int NB>
-__device__ inline void cut(float (&x)[8], Step<NB> &t, int32_t key, int32_t lo, int32_t hi, int32_t len, uint32_t g) {
+__device__ inline void cut_scales(Step<NB> &t, int32_t key, int32_t len, uint32_t r, uint32_t g) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 2; ++i) {
+    const int32_t k = key + 16 * i + 4 * (int32_t)g + 2 * (int32_t)(r & 1);
+    uint32_t keep = t.there[i] && k < len ? 0xffffu : 0;
+    if (t.there[i] && k + 1 < len) keep |= 0xffff0000u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int32_t k = key + 16 * i + 4 * (int32_t)g + j;
-      if (!(k >= lo && k < hi && t.there[i])) x[4 * i + j] = -__builtin_inff();
-      if (!(k < len && t.there[i])) {
+    for (int n = 0; n < Step<NB>::kScaleWords; ++n) t.s[i][n] &= keep;
+  }
+}
+template <int NB>
+__device__ inline void cut_scores(float (&x)[8], const Step<NB> &t, int32_t key, int32_t lo, int32_t hi, uint32_t g) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) t.vs[i][2 * b + j / 2] &= j % 2 ? 0x0000ffffu : 0xffff0000u;
-      }
-    }
+  for (int i = 0; i < 8; ++i) {
+    const int32_t k = key + 16 * (i / 4) + 4 * (int32_t)g + i % 4;
+    x[i] = k >= lo && k < hi && t.there[i / 4] ? x[i] : -__builtin_inff();
+  }
 }
 
 // Two f32 as f16 pairs: their roundings and what those leave (exact), rounded.
@@ -253,6 +315,27 @@ __device__ inline void split_pair(float minus1, float x, float y, uint32_t &hi, 
   const f32x2 r = {__builtin_fmaf((float)h.x, minus1, x), __builtin_fmaf((float)h.y, minus1, y)};
   hi = as_u32(h);
   lo = as_u32(__builtin_convertvector(r, f16x2));
+}
+
+// The words from 2 nb on are V's: only these are looked at here, as f32 numbers
+// (times 2^-e once that is known).
+template <int NB>
+struct VScales {
+  static constexpr int kFirst = 2 * NB / 16, kLane = 2 * NB % 16;
+  float s[2][Step<NB>::kScaleWords][2];  // [tile][word][half]
+  template <int I>
+  __device__ float of(int tile) const {  // V scale I = 4 b + token
+    constexpr int i = 4 * NB + I;
+    return from_lane<i / 2 % 16>(s[tile][i / 32][i % 2]);
+  }
+};
+
+template <int NB>
+__device__ inline void rescale(Acc<NB> &A, float f) {
+#pragma unroll
+  for (int n = 0; n < 2 * NB; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) A.o[n][j] *= f;
 }
 
 // Softmax weights of a step and their product with V.
@@ -268,43 +351,68 @@ __device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const St
     const float f = __builtin_amdgcn_exp2f(A.ref - ref);
     A.ref = ref;
     A.sum *= f;
-#pragma unroll
-    for (int n = 0; n < 2 * NB; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) A.o[n][j] *= f;
+    rescale(A, f);
   }
-  uint32_t hi[4], lo[4];
+  VScales<NB> c;
+  float big = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], fac, -A.ref));
-    const float x1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], fac, -A.ref));
-    A.sum += x0;
-    A.sum += x1;
-    split_pair(m.minus1, x0, x1, hi[i], lo[i]);
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int n = VScales<NB>::kFirst; n < Step<NB>::kScaleWords; ++n) {
+      const f16x2 w = as_f16x2(t.s[i][n]);
+      c.s[i][n][0] = (float)w.x;
+      c.s[i][n][1] = (float)w.y;
+      big = __builtin_fmaxf(big, __builtin_fmaxf(c.s[i][n][0], c.s[i][n][1]));
+    }
+  if (__any(big > A.most)) {  // (a lane of K scales has an infinite `most`)
+    const bool mine = (threadIdx.x & 15) >= VScales<NB>::kLane;
+    big = wave_max(mine ? big : 0.0f);
+    const float down = __builtin_ldexpf(1.0f, -__builtin_amdgcn_frexp_expf(big));
+    rescale(A, down / A.down);
+    A.down = down;
+    A.most = mine ? 2 / down : __builtin_inff();
   }
-  const f16x8 ph = as_f16x8(hi[0], hi[1], hi[2], hi[3]), pl = as_f16x8(lo[0], lo[1], lo[2], lo[3]);
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+  for (int i = 0; i < 8; ++i) {
+    x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], fac, -A.ref));
+    A.sum += x[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int n = VScales<NB>::kFirst; n < Step<NB>::kScaleWords; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) c.s[i][n][h] *= A.down;
+  each<NB>([&](auto B) {
+    constexpr int b = B();
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      each<2>([&](auto J) {
+        constexpr int j = J(), first = 4 * b + 2 * j;
+        const float p0 = c.template of<first>(i) * x[4 * i + 2 * j];
+        const float p1 = c.template of<first + 1>(i) * x[4 * i + 2 * j + 1];
+        if (P == 2) split_pair(m.minus1, p0, p1, ph[2 * i + j], pl[2 * i + j]);
+        else ph[2 * i + j] = as_u32(__builtin_convertvector(((f32x2){p0, p1}), f16x2));
+      });
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       // words hold tokens 0 2 1 3: (tok0, tok1) then (tok2, tok3)
-      uint32_t vh[4], vl[4];
+      uint32_t v[4];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t w = t.v[i][b] >> (8 * j);
-          const f16x2 n = half ? codes<true>(m, w) : codes<false>(m, w), s = as_f16x2(t.vs[i][2 * b + j]);
-          const f16x2 v = n * s;
-          vh[2 * i + j] = as_u32(v);
-          if (P == 2) vl[2 * i + j] = as_u32(__builtin_elementwise_fma(n, s, -v));
+          v[2 * i + j] = as_u32(half ? codes<true>(m, w) : codes<false>(m, w));
         }
+      const f16x8 v8 = as_f16x8(v[0], v[1], v[2], v[3]);
       f32x4 d = A.o[2 * b + half];
-      const f16x8 v8 = as_f16x8(vh[0], vh[1], vh[2], vh[3]);
-      d = mfma(v8, pl, d);
-      if (P == 2) d = mfma(as_f16x8(vl[0], vl[1], vl[2], vl[3]), ph, d);
-      A.o[2 * b + half] = mfma(v8, ph, d);
+      if (P == 2) d = mfma(v8, as_f16x8(pl[0], pl[1], pl[2], pl[3]), d);
+      A.o[2 * b + half] = mfma(v8, as_f16x8(ph[0], ph[1], ph[2], ph[3]), d);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  });
 }
 
 // The 32-key steps [first, first + steps) that some column of the tile sees,
@@ -342,7 +450,7 @@ __device__ inline void put<f16>(f16 *out, float v) { *out = (f16)v; }
 // of the workgroup's share; their results meet in LDS.  Grid: tiles of columns x
 // splits, kv heads, sequences.
 template <int NB, int W, typename T>
-__global__ __launch_bounds__(64 * W, NB == 8 ? 1 : 2) void kv4_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * W, NB == 8 ? 2 : 3) void kv4_attn_kernel(AttnArgs a) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
   constexpr int D = NB * 32;
   const uint32_t tile = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
@@ -380,6 +488,8 @@ __global__ __launch_bounds__(64 * W, NB == 8 ? 1 : 2) void kv4_attn_kernel(AttnA
   Acc<NB> A;
   A.ref = kNever;
   A.sum = 0;
+  A.down = 1;
+  A.most = r >= 2 * NB % 16 ? 0.0f : __builtin_inff();
 #pragma unroll
   for (int n = 0; n < 2 * NB; ++n) A.o[n] = (f32x4){0, 0, 0, 0};
 
@@ -394,21 +504,20 @@ __global__ __launch_bounds__(64 * W, NB == 8 ? 1 : 2) void kv4_attn_kernel(AttnA
   if (at < end) fetch<NB>(st[0], a.kv, pages, head, at * kKeys, lane);
   find_pages(pages, a.kv, seq, (at + W) * kKeys, at + W < end ? s.len : 0);
   while (at < end) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (at + W < end) fetch<NB>(st[1 - i], a.kv, pages, head, (at + W) * kKeys, lane);
-      find_pages(pages, a.kv, seq, (at + 2 * W) * kKeys, at + 2 * W < end ? s.len : 0);
-      const int32_t key = at * kKeys;
-      float x[8];
-      scores<NB, P>(x, Q, st[i], m);
-      if (key < all_lo || key + kKeys > all_hi || !st[i].there[0] || !st[i].there[1])
-        cut<NB>(x, st[i], key, lo, hi, s.len, g);
-      add_values<NB, P>(A, x, Q.fac, st[i], m);
-      at += W;
-      if (at >= end) break;
-    }
+    if (at + W < end) fetch<NB>(st[1], a.kv, pages, head, (at + W) * kKeys, lane);
+    find_pages(pages, a.kv, seq, (at + 2 * W) * kKeys, at + 2 * W < end ? s.len : 0);
+    const int32_t key = at * kKeys;
+    const bool whole = key >= all_lo && key + kKeys <= all_hi && st[0].there[0] && st[0].there[1];
+    if (!whole) cut_scales<NB>(st[0], key, s.len, r, g);
+    float x[8];
+    scores<NB, P>(x, Q, st[0], m);
+    if (!whole) cut_scores<NB>(x, st[0], key, lo, hi, g);
+    add_values<NB, P>(A, x, Q.fac, st[0], m);
+    st[0] = st[1];
+    at += W;
   }
   A.sum = sum_across(A.sum);
+  const float up = 1 / A.down;  // a power of two
 
   // the waves' results: a common reference, then sums over the waves
   __shared__ float sh_ref[W][kCols], sh_sum[W][kCols];
@@ -418,7 +527,7 @@ __global__ __launch_bounds__(64 * W, NB == 8 ? 1 : 2) void kv4_attn_kernel(AttnA
     sh_sum[wave][r] = A.sum;
   }
 #pragma unroll
-  for (int n = 0; n < 2 * NB; ++n) *reinterpret_cast<f32x4 *>(&sh_o[wave][r][16 * n + 4 * g]) = A.o[n];
+  for (int n = 0; n < 2 * NB; ++n) *reinterpret_cast<f32x4 *>(&sh_o[wave][r][16 * n + 4 * g]) = A.o[n] * up;
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < kCols * D; i += 64 * W) {
     const uint32_t c = i / D, d = i % D;
@@ -437,8 +546,7 @@ __global__ __launch_bounds__(64 * W, NB == 8 ? 1 : 2) void kv4_attn_kernel(AttnA
       put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + d, sum == 0 ? 0.0f : o / sum);
     } else {
       const uint32_t tiles = gridDim.x / a.splits;
-      float *w = a.work + ((((size_t)seq * gridDim.y + head) * tiles + tile) * a.splits + split) *
-                              (kCols * (D + 2));
+      float *w = a.work + ((((size_t)seq * gridDim.y + head) * tiles + tile) * a.splits + split) * kShare<D>;
       w[i] = o;
       if (d == 0) {
         w[kCols * D + c] = ref;
@@ -448,32 +556,49 @@ __global__ __launch_bounds__(64 * W, NB == 8 ? 1 : 2) void kv4_attn_kernel(AttnA
   }
 }
 
-// The splits' results of one tile of columns, joined.  A workgroup per tile,
-// kv head and sequence.
+// The shares' results of one column, joined: a workgroup per column, kv head
+// and sequence.  The shares' references and sums first (a thread each), then
+// D threads add up the shares' O, 256 / D groups of them every so many shares.
 template <int NB, typename T>
-__global__ __launch_bounds__(256) void kv4_attn_join_kernel(AttnArgs a) {
-  constexpr int D = NB * 32;
-  const uint32_t tile = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
+__global__ __launch_bounds__(256) void kv4_attn_join_kernel(AttnArgs a, uint32_t tiles, uint32_t tile_cols) {
+  constexpr int D = NB * 32, G = 256 / D;
+  const uint32_t tile = blockIdx.x / tile_cols, c = blockIdx.x % tile_cols, head = blockIdx.y, seq = blockIdx.z;
   const Kv4Seq s = kv4_seq(a.kv, seq);
   const uint32_t cols = s.nrows * a.group, col0 = tile * kCols;
-  if (col0 >= cols) return;
+  if (col0 + c >= cols) return;
   const Range rg = key_range(a, s, col0, cols);
   if (rg.active == 1) return;
-  const float *w = a.work + (((size_t)seq * gridDim.y + head) * gridDim.x + tile) * a.splits * (kCols * (D + 2));
-  for (uint32_t i = threadIdx.x; i < kCols * D; i += 256) {
-    const uint32_t c = i / D, d = i % D;
-    if (col0 + c >= cols) break;
-    float ref = kNever, o = 0, sum = 0;
-    for (int32_t n = 0; n < rg.active; ++n)
-      ref = __builtin_fmaxf(ref, w[(size_t)n * (kCols * (D + 2)) + kCols * D + c]);
-    for (int32_t n = 0; n < rg.active; ++n) {
-      const float *p = w + (size_t)n * (kCols * (D + 2));
-      const float f = __builtin_amdgcn_exp2f(p[kCols * D + c] - ref);
-      sum = __builtin_fmaf(p[kCols * D + kCols + c], f, sum);
-      o = __builtin_fmaf(p[i], f, o);
-    }
+  const float *w = a.work + (((size_t)seq * gridDim.y + head) * tiles + tile) * a.splits * kShare<D>;
+  __shared__ float weight[kMaxSplits], part[G][D], red[8];
+  const uint32_t t = threadIdx.x;
+  static_assert(kMaxSplits <= 256, "a thread per share");
+  const bool mine = (int32_t)t < rg.active;
+  const float ref = mine ? w[t * kShare<D> + kCols * D + c] : kNever;
+  const float sum = mine ? w[t * kShare<D> + kCols * D + kCols + c] : 0;
+  const float top = wave_max(ref);
+  if (t % 64 == 0) red[t / 64] = top;
+  __syncthreads();
+  const float f = __builtin_amdgcn_exp2f(ref - __builtin_fmaxf(__builtin_fmaxf(red[0], red[1]),
+                                                               __builtin_fmaxf(red[2], red[3])));
+  const float all = wave_sum(sum * f);
+  if (t % 64 == 0) red[4 + t / 64] = all;
+  if (mine) weight[t] = f;
+  __syncthreads();
+  const uint32_t grp = t / D, d = t % D;
+  if (grp < G) {
+    float o = 0;
+#pragma unroll 8
+    for (int32_t n = grp; n < rg.active; n += G) o = __builtin_fmaf(w[n * kShare<D> + c * D + d], weight[n], o);
+    part[grp][d] = o;
+  }
+  __syncthreads();
+  if (t < D) {
+    float o = 0;
+#pragma unroll
+    for (int g = 0; g < G; ++g) o += part[g][t];
+    const float l = (red[4] + red[5]) + (red[6] + red[7]);
     const uint32_t orow = s.row0 + (col0 + c) / a.group, oh = head * a.group + (col0 + c) % a.group;
-    put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + d, sum == 0 ? 0.0f : o / sum);
+    put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + t, l == 0 ? 0.0f : o / l);
   }
 }
 
@@ -481,30 +606,34 @@ struct Plan {
   uint32_t tiles, splits, min_steps;
   size_t share;  // bytes of one split of one tile
 };
-// How many workgroups share the keys of a tile: enough for two workgroups per
-// CU, none with less than eight steps (a step per wave twice).
+// How many workgroups may share the keys of a tile, and the fewest steps of a
+// share: two workgroups per CU if every sequence had len_max keys, but shares
+// of no more than 64 steps (a batch's lengths may differ; the long ones must
+// not be what the call waits for) and of no less than 8 (two per wave).
 Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, uint32_t cus) {
   Plan p;
   const uint64_t reach = (uint64_t)b->max_pages * c->page;
   const uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
   const uint64_t cols = (uint64_t)b->rows * (nh / c->nkv);
   p.tiles = (uint32_t)((cols + kCols - 1) / kCols);
-  p.min_steps = 8;
   p.share = (size_t)kCols * (c->d + 2) * 4;
   const uint64_t groups = (uint64_t)p.tiles * c->nkv * b->b, steps = (len + kKeys - 1) / kKeys;
-  uint64_t want = groups ? (2ull * cus + groups - 1) / groups : 1;
-  const uint64_t most = steps / p.min_steps;
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  if (want > 256) want = 256;
-  p.splits = (uint32_t)want;
+  uint64_t per = groups * steps / (2 * cus);
+  per = per > 64 ? 64 : per < 8 ? 8 : per;
+  uint64_t want = (steps + per - 1) / per;
+  if (groups >= 8ull * cus) want = 1;
+  p.min_steps = (uint32_t)per;
+  p.splits = (uint32_t)(want > kMaxSplits ? kMaxSplits : want < 1 ? 1 : want);
   return p;
 }
 
 template <int NB, typename T>
 void launch(const AttnArgs &a, uint32_t tiles, uint32_t b) {
   kv4_attn_kernel<NB, 4, T><<<dim3(tiles * a.splits, a.kv.nkv, b), 256, 0, stream()>>>(a);
-  if (a.splits > 1) kv4_attn_join_kernel<NB, T><<<dim3(tiles, a.kv.nkv, b), 256, 0, stream()>>>(a);
+  const uint64_t cols = (uint64_t)a.kv.rows * a.group;
+  const uint32_t tile_cols = cols < kCols ? (uint32_t)cols : kCols;
+  if (a.splits > 1)
+    kv4_attn_join_kernel<NB, T><<<dim3(tiles * tile_cols, a.kv.nkv, b), 256, 0, stream()>>>(a, tiles, tile_cols);
 }
 
 }  // namespace
