@@ -28,6 +28,11 @@ inline bool kv4_overlap(const void *a, size_t an, const void *b, size_t bn) {
 }
 
 // ---------------------------------------------------------------- device side
+// A number that no kernel writes while others read it: at a uniform address one
+// scalar load, whatever else the kernel stores.
+__device__ inline uint32_t kv4_const(const uint32_t *p) {
+  return *(const __attribute__((address_space(4))) uint32_t *)(uintptr_t)p;
+}
 // One sequence of the batch: its length, its rows [row0, row0 + nrows) of the
 // inputs and outputs, and the position of the first.
 struct Kv4Seq {
@@ -36,12 +41,12 @@ struct Kv4Seq {
 };
 __device__ inline Kv4Seq kv4_seq(const Kv4Args &a, uint32_t i) {
   Kv4Seq s;
-  const uint32_t reach = a.max_pages << a.shift, len = a.lens[i];
+  const uint32_t reach = a.max_pages << a.shift, len = kv4_const(a.lens + i);
   s.len = (int32_t)(len < reach ? len : reach);
   uint32_t lo = i * a.rows, hi = lo + a.rows;
   if (a.row_off) {
-    lo = a.row_off[i];
-    hi = a.row_off[i + 1];
+    lo = kv4_const(a.row_off + i);
+    hi = kv4_const(a.row_off + i + 1);
   }
   hi = hi < a.m ? hi : a.m;
   lo = lo < hi ? lo : hi;
@@ -53,7 +58,7 @@ __device__ inline Kv4Seq kv4_seq(const Kv4Args &a, uint32_t i) {
 }
 // Page of position pos (0 <= pos < reach) of sequence i.
 __device__ inline uint32_t kv4_page(const Kv4Args &a, uint32_t i, uint32_t pos) {
-  return a.table[(size_t)i * a.max_pages + (pos >> a.shift)];
+  return kv4_const(a.table + (size_t)i * a.max_pages + (pos >> a.shift));
 }
 // Bytes of one page and head, and the start of page p, head h.
 __device__ inline size_t kv4_block_bytes(uint32_t shift, uint32_t d) {

@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "kv4.h"
+#include "vmem.h"
 
 using namespace madi;
 
@@ -36,27 +37,33 @@ constexpr float kNever = -1e30f;  // reference before any key was seen
 // rounds to nothing is 2^-32 of the largest P at the largest s.
 constexpr float kLift = 7.0f, kRaise = 14.0f;
 
-constexpr int kMaxSplits = 256;
-// f32 numbers of a share: O [16][D], then the references and the sums.
+// What a segment costs beside its steps (finding it, its queries, the first
+// words' latency, the waves' results put together), in steps.
+constexpr uint32_t kOverhead = 8;
+// Workgroups that share the steps, at most.
+constexpr uint32_t kMaxGroups = 1024;
+// f32 numbers of a partial result: O [16][D], then the references and the sums.
 template <int D>
 constexpr size_t kShare = kCols * (D + 2);
+
+// Workgroups of four waves that a CU holds at once, by registers (f32 rows: those of
+// the low parts) and by LDS (the ring).
+constexpr uint32_t resident(uint32_t d, bool f32) { return d == 256 ? 2 : f32 && d == 128 ? 3 : 4; }
 
 struct AttnArgs {
   Kv4Args kv;
   const void *q;
   void *out;
-  float *work;
-  uint32_t ldq, ldo, group, window, causal, splits, min_steps;
+  float *work;         // partial results, two per workgroup
+  uint32_t *starts;    // behind them: the items' starts, and the length of a share
+  uint32_t ldq, ldo, group, window, causal;
+  uint32_t tiles, items;  // column tiles of a sequence; tiles of all sequences
+  uint32_t shared;        // the steps are dealt out evenly (else a workgroup per tile and head)
   float scale;
 };
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-template <int N>
-__device__ inline void load_words(const uint8_t *p, uint32_t (&w)[N]) {
-  constexpr int A = N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4;
-  __builtin_memcpy(w, __builtin_assume_aligned(p, A), 4 * N);
-}
 __device__ inline f16x2 as_f16x2(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
 __device__ inline uint32_t as_u32(f16x2 v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ inline f16x8 as_f16x8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -126,29 +133,78 @@ __device__ inline void find_pages(uint32_t (&page)[2], const Kv4Args &a, uint32_
   for (int i = 0; i < 2; ++i) page[i] = key + 16 * i < len ? kv4_page(a, seq, key + 16 * i) : 0xffffffffu;
 }
 
+// A wave's ring of steps in LDS.  Every lane reads back what it loaded itself,
+// so a wave waits for its own loads only, and in registers there is one step.
+// Words of K, V and scales of a tile as pieces of 16 (4 for what is left) bytes
+// per lane; a piece's 64 lanes lie side by side.
 template <int NB>
-__device__ inline void fetch(Step<NB> &t, const Kv4Args &a, const uint32_t (&pages)[2], uint32_t head, int32_t key,
-                             uint32_t lane) {
+struct Ring {
+  static constexpr int kDepth = NB == 2 ? 4 : 2;
+  static constexpr int kWide = NB / 4, kNarrow = NB % 4;  // pieces of NB words
+  static constexpr int kScales = Step<NB>::kScaleWords;
+  static constexpr int kTile = 256 * (2 * NB + kScales), kBytes = 2 * kTile;
+  static constexpr int kLoads = 2 * (2 * (kWide + kNarrow) + kScales);  // of a step
+};
+template <int NB>
+__device__ inline void load_pieces(const uint8_t *from, uint32_t voff, uint32_t to) {
+#pragma unroll
+  for (int n = 0; n < Ring<NB>::kWide; ++n) global_dma<16>(from + 16 * n, voff, to + 1024 * n);
+#pragma unroll
+  for (int n = 0; n < Ring<NB>::kNarrow; ++n)
+    global_dma<4>(from + 16 * Ring<NB>::kWide + 4 * n, voff, to + 1024 * Ring<NB>::kWide + 256 * n);
+}
+template <int NB>
+__device__ inline void read_pieces(uint32_t (&w)[NB], const uint8_t *from, uint32_t lane) {
+#pragma unroll
+  for (int n = 0; n < Ring<NB>::kWide; ++n) {
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(from + 1024 * n + 16 * lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[4 * n + i] = v[i];
+  }
+#pragma unroll
+  for (int n = 0; n < Ring<NB>::kNarrow; ++n)
+    w[4 * Ring<NB>::kWide + n] =
+        *reinterpret_cast<const uint32_t *>(from + 1024 * Ring<NB>::kWide + 256 * n + 4 * lane);
+}
+// Starts the loads of the step at `key` into the ring's slot at LDS address
+// `to`; returns which tiles have a page (bits 0 and 1).
+template <int NB>
+__device__ inline uint32_t fetch(const Kv4Args &a, const uint32_t (&pages)[2], uint32_t head, int32_t key, uint32_t lane,
+                                 uint32_t to) {
   constexpr uint32_t D = NB * 32;
   const uint32_t r = lane & 15, g = lane >> 4;
+  uint32_t there = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     // a tile without a page: any valid one stands in
-    t.there[i] = pages[i] < a.n_pages;
-    const uint32_t page = t.there[i] ? pages[i] : 0;
+    const bool ok = pages[i] < a.n_pages;
+    there |= ok ? 1u << i : 0;
     const uint32_t off = (uint32_t)(key + 16 * i) & ((1u << a.shift) - 1);
-    const uint8_t *blk = kv4_block(a, page, head, D);
-    const uint8_t *kp = blk + (size_t)off * (D / 2) + (r * (D / 2) + g * (4 * NB));
-    const uint8_t *vp = blk + ((size_t)(D / 2) << a.shift) + (size_t)(off / 4) * (2 * D) + (g * (2 * D) + r * (4 * NB));
-    const uint8_t *sp = blk + ((size_t)D << a.shift) + (size_t)(off / 4) * (D / 2) + g * (D / 2);
-    constexpr uint32_t kWords = 4 * NB;  // of a group
-    load_words<NB>(kp, t.k[i]);
-    load_words<NB>(vp, t.v[i]);
+    const uint8_t *blk = kv4_block(a, ok ? pages[i] : 0, head, D);
+    const uint8_t *v = blk + ((size_t)(D / 2) << a.shift) + (size_t)off * (D / 2);
+    const uint8_t *sc = blk + ((size_t)D << a.shift) + (size_t)off * (D / 8);
+    const uint32_t at = to + i * Ring<NB>::kTile;
+    load_pieces<NB>(blk + (size_t)off * (D / 2), r * (D / 2) + g * (4 * NB), at);
+    load_pieces<NB>(v, g * (2 * D) + r * (4 * NB), at + 256 * NB);
 #pragma unroll
-    for (uint32_t n = 0; n < Step<NB>::kScaleWords; ++n) {
+    for (uint32_t n = 0; n < Ring<NB>::kScales; ++n) {
       const uint32_t w = 16 * n + r;  // (nb < 4: lanes past the words hold the last one)
-      load_words<1>(sp + 4 * (w < kWords ? w : kWords - 1), *reinterpret_cast<uint32_t(*)[1]>(&t.s[i][n]));
+      global_dma<4>(sc, g * (D / 2) + 4 * (w < 4 * NB ? w : 4 * NB - 1), at + 512 * NB + 256 * n);
     }
+  }
+  return there;
+}
+template <int NB>
+__device__ inline void read_step(Step<NB> &t, const uint8_t *slot, uint32_t there, uint32_t lane) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint8_t *at = slot + i * Ring<NB>::kTile;
+    read_pieces<NB>(t.k[i], at, lane);
+    read_pieces<NB>(t.v[i], at + 256 * NB, lane);
+#pragma unroll
+    for (int n = 0; n < Ring<NB>::kScales; ++n)
+      t.s[i][n] = *reinterpret_cast<const uint32_t *>(at + 512 * NB + 256 * n + 4 * lane);
+    t.there[i] = there >> i & 1;
   }
 }
 
@@ -415,28 +471,38 @@ __device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const St
   });
 }
 
-// The 32-key steps [first, first + steps) that some column of the tile sees,
-// and the split of them over workgroups: `per` steps each, `active` shares.
-struct Range {
-  int32_t first, steps, per, active;
+// A tile of 16 columns of a sequence, and the 32-key steps [first, first + steps)
+// that some column of it sees.
+struct Item {
+  Kv4Seq s;
+  uint32_t seq, cols, col0;  // the sequence's columns, the tile's first
+  int32_t first, steps;
+  bool none;                 // past the sequence's columns
 };
-__device__ inline Range key_range(const AttnArgs &a, const Kv4Seq &s, uint32_t col0, uint32_t cols) {
-  Range r;
-  int32_t lo = 0, hi = s.len;
+__device__ inline Item item_of(const AttnArgs &a, uint32_t item) {
+  Item t;
+  t.seq = a.tiles == 1 ? item : item / a.tiles;
+  t.col0 = (item - t.seq * a.tiles) * kCols;
+  t.s = kv4_seq(a.kv, t.seq);
+  t.cols = t.s.nrows * a.group;
+  t.none = t.col0 >= t.cols;
+  int32_t lo = 0, hi = t.s.len;
   if (a.causal) {
-    const uint32_t last = (col0 + kCols < cols ? col0 + kCols : cols) - 1;
-    const int32_t p0 = s.pos0 + (int32_t)(col0 / a.group), p1 = s.pos0 + (int32_t)(last / a.group);
+    const uint32_t last = (t.col0 + kCols < t.cols ? t.col0 + kCols : t.cols) - 1;
+    const int32_t p0 = t.s.pos0 + (int32_t)(t.col0 / a.group), p1 = t.s.pos0 + (int32_t)(last / a.group);
     hi = p1 + 1 < hi ? p1 + 1 : hi;
     if (a.window && p0 >= (int32_t)a.window) lo = p0 - (int32_t)a.window + 1;
   }
-  hi = hi > 0 ? hi : 0;
-  r.first = lo / kKeys;
-  r.steps = (hi + kKeys - 1) / kKeys - r.first;
-  r.steps = r.steps > 0 ? r.steps : 0;
-  const int32_t even = (r.steps + (int32_t)a.splits - 1) / (int32_t)a.splits;
-  r.per = even > (int32_t)a.min_steps ? even : (int32_t)a.min_steps;
-  r.active = r.steps ? (r.steps + r.per - 1) / r.per : 1;
-  return r;
+  hi = hi > 0 && !t.none ? hi : 0;
+  t.first = lo / kKeys;
+  t.steps = (hi + kKeys - 1) / kKeys - t.first;
+  t.steps = t.steps > 0 ? t.steps : 0;
+  return t;
+}
+// Length of an item (all its heads) in the row of all items: a head's steps come
+// after kOverhead places of none.
+__device__ inline uint32_t item_length(const AttnArgs &a, const Item &t) {
+  return t.none ? 0 : ((uint32_t)t.steps + kOverhead) * a.kv.nkv;
 }
 
 template <typename T>
@@ -446,194 +512,330 @@ __device__ inline void put<float>(float *out, float v) { *out = v; }
 template <>
 __device__ inline void put<f16>(f16 *out, float v) { *out = (f16)v; }
 
-// Workgroup: W waves on the same 16 columns, wave w taking steps w, w + W, ..
-// of the workgroup's share; their results meet in LDS.  Grid: tiles of columns x
-// splits, kv heads, sequences.
+// Sum over the workgroup's threads before the caller, and over all.
+template <int W>
+__device__ inline uint32_t scan(uint32_t v, uint32_t &all, uint32_t *lds) {
+  uint32_t x = v;
+  const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+  for (uint32_t n = 1; n < 64; n *= 2) {
+    const uint32_t y = __shfl_up(x, n);
+    x += lane >= n ? y : 0;
+  }
+  __syncthreads();
+  if (lane == 63) lds[threadIdx.x / 64] = x;
+  __syncthreads();
+  all = 0;
+  uint32_t before = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < W; ++w) {
+    before += w < threadIdx.x / 64 ? lds[w] : 0;
+    all += lds[w];
+  }
+  return before + x - v;
+}
+
+// W waves on the same 16 columns, wave w taking steps w, w + W, .. of the
+// workgroup's segments.
+//
+// shared: the steps of all items and heads in a row (item by item, head by
+// head, each after kOverhead empty places) are dealt out to the workgroups in
+// equal shares, however long the sequences are; a share may hold several
+// segments, and a segment that is not a whole item and head goes into the workspace
+// for kv4_attn_join_kernel.  A workgroup has two places there: 0 for
+// a segment that others began, 1 for one that it begins and does not end.
+// Else: a workgroup per item and head.
 template <int NB, int W, typename T>
-__global__ __launch_bounds__(64 * W, NB == 8 ? 2 : 3) void kv4_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4_attn_kernel(AttnArgs a) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
   constexpr int D = NB * 32;
-  const uint32_t tile = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
-  const uint32_t head = blockIdx.y, seq = blockIdx.z;
-  const Kv4Seq s = kv4_seq(a.kv, seq);
-  const uint32_t cols = s.nrows * a.group, col0 = tile * kCols;
-  if (col0 >= cols) return;
-  const Range rg = key_range(a, s, col0, cols);
-  if ((int32_t)split >= rg.active) return;
+  constexpr int R = Ring<NB>::kDepth;
+  struct Results {
+    float ref[W][kCols], sum[W][kCols], o[W][kCols][D + 4];
+  };
+  constexpr size_t kLds = sizeof(Results) > (size_t)W * R * Ring<NB>::kBytes ? sizeof(Results)
+                                                                             : (size_t)W * R * Ring<NB>::kBytes;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+  uint32_t *found = reinterpret_cast<uint32_t *>(lds);  // before the ring is used
+  Results &res = *reinterpret_cast<Results *>(lds);
 
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t r = lane & 15, g = lane >> 4, col = col0 + r;
-  const bool mine = col < cols;
-  const uint32_t row = mine ? col / a.group : 0, sub = mine ? col % a.group : 0;
-  Query<NB, P> Q;
-  load_query<NB, P, T>(Q, static_cast<const T *>(a.q) + (size_t)(s.row0 + row) * a.ldq +
-                              (size_t)(head * a.group + sub) * D, mine, g, a.scale);
-  // keys the lane's column sees
-  int32_t lo = 0, hi = s.len;
-  if (a.causal) {
-    const int32_t p = s.pos0 + (int32_t)row;
-    hi = p + 1 < hi ? p + 1 : hi;
-    if (a.window && p >= (int32_t)a.window) lo = p - (int32_t)a.window + 1;
-  }
-  if (!mine) hi = 0;
-  // keys every column of the wave sees
-  int32_t all_lo = 0, all_hi = s.len;
-  if (a.causal) {
-    const uint32_t last = (col0 + kCols < cols ? col0 + kCols : cols) - 1;
-    const int32_t p0 = s.pos0 + (int32_t)(col0 / a.group), p1 = s.pos0 + (int32_t)(last / a.group);
-    all_hi = p0 + 1 < all_hi ? p0 + 1 : all_hi;
-    if (a.window && p1 >= (int32_t)a.window) all_lo = p1 - (int32_t)a.window + 1;
-  }
-
-  Acc<NB> A;
-  A.ref = kNever;
-  A.sum = 0;
-  A.down = 1;
-  A.most = r >= 2 * NB % 16 ? 0.0f : __builtin_inff();
-#pragma unroll
-  for (int n = 0; n < 2 * NB; ++n) A.o[n] = (f32x4){0, 0, 0, 0};
-
-  const int32_t end = rg.first + (((int32_t)split + 1) * rg.per < rg.steps ? ((int32_t)split + 1) * rg.per : rg.steps);
-  int32_t at = rg.first + (int32_t)split * rg.per + (int32_t)wave;
-  // Two steps' words in registers, one used while the other arrives, and the
-  // page numbers one step further ahead.
-  Step<NB> st[2];
-  uint32_t pages[2];
+  const uint32_t r = lane & 15, g = lane >> 4;
+  const uint8_t *ring = lds + wave * (R * Ring<NB>::kBytes);
+  const uint32_t ring_at = lds_addr(ring);
   const Masks m = masks();
-  find_pages(pages, a.kv, seq, at * kKeys, at < end ? s.len : 0);
-  if (at < end) fetch<NB>(st[0], a.kv, pages, head, at * kKeys, lane);
-  find_pages(pages, a.kv, seq, (at + W) * kKeys, at + W < end ? s.len : 0);
-  while (at < end) {
-    if (at + W < end) fetch<NB>(st[1], a.kv, pages, head, (at + W) * kKeys, lane);
-    find_pages(pages, a.kv, seq, (at + 2 * W) * kKeys, at + 2 * W < end ? s.len : 0);
-    const int32_t key = at * kKeys;
-    const bool whole = key >= all_lo && key + kKeys <= all_hi && st[0].there[0] && st[0].there[1];
-    if (!whole) cut_scales<NB>(st[0], key, s.len, r, g);
-    float x[8];
-    scores<NB, P>(x, Q, st[0], m);
-    if (!whole) cut_scores<NB>(x, st[0], key, lo, hi, g);
-    add_values<NB, P>(A, x, Q.fac, st[0], m);
-    st[0] = st[1];
-    at += W;
-  }
-  A.sum = sum_across(A.sum);
-  const float up = 1 / A.down;  // a power of two
 
-  // the waves' results: a common reference, then sums over the waves
-  __shared__ float sh_ref[W][kCols], sh_sum[W][kCols];
-  __shared__ float sh_o[W][kCols][D + 4];
-  if (g == 0) {
-    sh_ref[wave][r] = A.ref;
-    sh_sum[wave][r] = A.sum;
-  }
-#pragma unroll
-  for (int n = 0; n < 2 * NB; ++n) *reinterpret_cast<f32x4 *>(&sh_o[wave][r][16 * n + 4 * g]) = A.o[n] * up;
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < kCols * D; i += 64 * W) {
-    const uint32_t c = i / D, d = i % D;
-    if (col0 + c >= cols) break;
-    float ref = kNever, o = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) ref = __builtin_fmaxf(ref, sh_ref[w][c]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sh_ref[w][c] - ref);
-      sum = __builtin_fmaf(sh_sum[w][c], f, sum);
-      o = __builtin_fmaf(sh_o[w][c][d], f, o);
+  // The workgroup's part [at, end) of the row, from place `in` of item `item`
+  uint32_t item, in, left;
+  if (a.shared) {
+    // the length of all items, then the one that holds place `from` (up to as
+    // many items as threads, both from one scan)
+    uint32_t total = 0, all, len = 0, start = 0;
+    for (uint32_t i = 0; i < a.items; i += 64 * W) {
+      const uint32_t n = i + threadIdx.x;
+      len = n < a.items ? item_length(a, item_of(a, n)) : 0;
+      start = total + scan<W>(len, all, found + 2);
+      total += all;
     }
-    if (rg.active == 1) {
-      const uint32_t orow = s.row0 + (col0 + c) / a.group, oh = head * a.group + (col0 + c) % a.group;
-      put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + d, sum == 0 ? 0.0f : o / sum);
-    } else {
-      const uint32_t tiles = gridDim.x / a.splits;
-      float *w = a.work + ((((size_t)seq * gridDim.y + head) * tiles + tile) * a.splits + split) * kShare<D>;
-      w[i] = o;
-      if (d == 0) {
-        w[kCols * D + c] = ref;
-        w[kCols * D + kCols + c] = sum;
+    uint32_t share = (total + gridDim.x - 1) / gridDim.x;
+    share = share > kOverhead + W ? share : kOverhead + W;
+    const uint32_t from = blockIdx.x * share;  // below total + share
+    if (threadIdx.x == 0) found[0] = a.items;
+    __syncthreads();
+    uint32_t base = 0;
+    for (uint32_t i = 0; i < a.items; i += 64 * W) {
+      const uint32_t n = i + threadIdx.x;
+      if (a.items > 64 * W) {
+        len = n < a.items ? item_length(a, item_of(a, n)) : 0;
+        start = base + scan<W>(len, all, found + 2);
+        base += all;
       }
+      if (from >= start && from - start < len) {
+        found[0] = n;
+        found[1] = from - start;
+      }
+      if (blockIdx.x == 0 && n < a.items) a.starts[1 + n] = start;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.starts[0] = share;
+    __syncthreads();
+    item = __builtin_amdgcn_readfirstlane(found[0]);
+    in = __builtin_amdgcn_readfirstlane(found[1]);
+    left = share;
+    __syncthreads();
+  } else {
+    item = blockIdx.x / a.kv.nkv;
+    in = blockIdx.x % a.kv.nkv;  // of heads
+    left = 1;
+  }
+
+  for (; item < a.items && left; ++item, in = 0) {
+    const Item t = item_of(a, item);
+    const Kv4Seq &s = t.s;
+    if (t.none) {
+      if (a.shared) continue;
+      return;
+    }
+    // keys every column of the tile sees
+    int32_t all_lo = 0, all_hi = s.len;
+    if (a.causal) {
+      const uint32_t last = (t.col0 + kCols < t.cols ? t.col0 + kCols : t.cols) - 1;
+      const int32_t p0 = s.pos0 + (int32_t)(t.col0 / a.group), p1 = s.pos0 + (int32_t)(last / a.group);
+      all_hi = p0 + 1 < all_hi ? p0 + 1 : all_hi;
+      if (a.window && p1 >= (int32_t)a.window) all_lo = p1 - (int32_t)a.window + 1;
+    }
+    // the lane's column: its row, head and keys [lo, hi)
+    const uint32_t col = t.col0 + r;
+    const bool mine = col < t.cols;
+    const uint32_t row = mine ? col / a.group : 0, sub = mine ? col % a.group : 0;
+    int32_t lo = 0, hi = s.len;
+    if (a.causal) {
+      const int32_t p = s.pos0 + (int32_t)row;
+      hi = p + 1 < hi ? p + 1 : hi;
+      if (a.window && p >= (int32_t)a.window) lo = p - (int32_t)a.window + 1;
+    }
+    if (!mine) hi = 0;
+
+    const uint32_t length = (uint32_t)t.steps + kOverhead;
+    uint32_t head = a.shared ? in / length : in, place = a.shared ? in - head * length : 0;
+    for (; head < a.kv.nkv && left; ++head, place = 0) {
+      // the segment: steps [begin, end) of the head's t.steps
+      int32_t begin = 0, end = t.steps;
+      bool last = true;  // of the head
+      if (a.shared) {
+        const uint32_t n = length - place < left ? length - place : left;
+        last = place + n == length;
+        begin = place > kOverhead ? (int32_t)(place - kOverhead) : 0;
+        end = place + n > kOverhead ? (int32_t)(place + n - kOverhead) : 0;
+        left -= n;
+        if (begin >= end && !(last && t.steps == 0)) continue;
+      } else {
+        left = 0;
+      }
+      const bool whole_head = begin == 0 && end == t.steps;
+
+      int32_t at = begin + (int32_t)wave, issued = at;
+      uint32_t slot_in = 0, there_in = 0;  // next slot to load; which tiles of the ring's slots have pages
+      uint32_t pages[2];
+      find_pages(pages, a.kv, t.seq, (t.first + issued) * kKeys, issued < end ? s.len : 0);
+      auto issue = [&]() {
+        if (issued < end) {
+          const uint32_t ok = fetch<NB>(a.kv, pages, head, (t.first + issued) * kKeys, lane,
+                                        ring_at + slot_in * Ring<NB>::kBytes);
+          there_in = (there_in & ~(3u << (2 * slot_in))) | ok << (2 * slot_in);
+          slot_in = slot_in + 1 == R ? 0 : slot_in + 1;
+          issued += W;
+          find_pages(pages, a.kv, t.seq, (t.first + issued) * kKeys, issued < end ? s.len : 0);
+        }
+      };
+#pragma unroll 1
+      for (int n = 0; n < R - 1; ++n) issue();
+
+      Query<NB, P> Q;
+      load_query<NB, P, T>(Q, static_cast<const T *>(a.q) + (size_t)(s.row0 + row) * a.ldq +
+                                  (size_t)(head * a.group + sub) * D, mine, g, a.scale);
+      Acc<NB> A;
+      A.ref = kNever;
+      A.sum = 0;
+      A.down = 1;
+      A.most = r >= 2 * NB % 16 ? 0.0f : __builtin_inff();
+#pragma unroll
+      for (int n = 0; n < 2 * NB; ++n) A.o[n] = (f32x4){0, 0, 0, 0};
+
+      uint32_t slot = 0;
+      while (at < end) {
+        issue();
+        // this step's loads are done when only those of the later ones are not
+        const int32_t later = (issued - at) / W - 1;
+        if (R > 3 && later == 3) wait_loads<3 * Ring<NB>::kLoads>();
+        else if (R > 2 && later == 2) wait_loads<2 * Ring<NB>::kLoads>();
+        else if (later == 1) wait_loads<Ring<NB>::kLoads>();
+        else wait_loads<0>();
+        Step<NB> st;
+        read_step<NB>(st, ring + slot * Ring<NB>::kBytes, there_in >> (2 * slot), lane);
+        slot = slot + 1 == R ? 0 : slot + 1;
+        const int32_t key = (t.first + at) * kKeys;
+        const bool whole = key >= all_lo && key + kKeys <= all_hi && st.there[0] && st.there[1];
+        if (!whole) cut_scales<NB>(st, key, s.len, r, g);
+        float x[8];
+        scores<NB, P>(x, Q, st, m);
+        if (!whole) cut_scores<NB>(x, st, key, lo, hi, g);
+        add_values<NB, P>(A, x, Q.fac, st, m);
+        at += W;
+      }
+      A.sum = sum_across(A.sum);
+      const float up = 1 / A.down;  // a power of two
+
+      // the waves' results: a common reference, then sums over the waves
+      __syncthreads();
+      if (g == 0) {
+        res.ref[wave][r] = A.ref;
+        res.sum[wave][r] = A.sum;
+      }
+      if (mine)
+#pragma unroll
+        for (int n = 0; n < 2 * NB; ++n) *reinterpret_cast<f32x4 *>(&res.o[wave][r][16 * n + 4 * g]) = A.o[n] * up;
+      __syncthreads();
+      const uint32_t ncols = t.cols - t.col0 < kCols ? t.cols - t.col0 : kCols;
+      float *part = a.work + (2 * (size_t)blockIdx.x + (begin == 0)) * kShare<D>;
+      for (uint32_t i = threadIdx.x; i < ncols * D; i += 64 * W) {
+        const uint32_t c = i / D, d = i % D;
+        float ref = kNever, o = 0, sum = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) ref = __builtin_fmaxf(ref, res.ref[w][c]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float f = __builtin_amdgcn_exp2f(res.ref[w][c] - ref);
+          sum = __builtin_fmaf(res.sum[w][c], f, sum);
+          o = __builtin_fmaf(res.o[w][c][d], f, o);
+        }
+        if (whole_head) {
+          const uint32_t orow = s.row0 + (t.col0 + c) / a.group, oh = head * a.group + (t.col0 + c) % a.group;
+          put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + d, sum == 0 ? 0.0f : o / sum);
+        } else {
+          part[i] = o;
+          if (d == 0) {
+            part[kCols * D + c] = ref;
+            part[kCols * D + kCols + c] = sum;
+          }
+        }
+      }
+      __syncthreads();
     }
   }
 }
 
-// The shares' results of one column, joined: a workgroup per column, kv head
-// and sequence.  The shares' references and sums first (a thread each), then
-// D threads add up the shares' O, 256 / D groups of them every so many shares.
-template <int NB, typename T>
-__global__ __launch_bounds__(256) void kv4_attn_join_kernel(AttnArgs a, uint32_t tiles, uint32_t tile_cols) {
-  constexpr int D = NB * 32, G = 256 / D;
-  const uint32_t tile = blockIdx.x / tile_cols, c = blockIdx.x % tile_cols, head = blockIdx.y, seq = blockIdx.z;
-  const Kv4Seq s = kv4_seq(a.kv, seq);
-  const uint32_t cols = s.nrows * a.group, col0 = tile * kCols;
-  if (col0 + c >= cols) return;
-  const Range rg = key_range(a, s, col0, cols);
-  if (rg.active == 1) return;
-  const float *w = a.work + (((size_t)seq * gridDim.y + head) * tiles + tile) * a.splits * kShare<D>;
-  __shared__ float weight[kMaxSplits], part[G][D], red[8];
-  const uint32_t t = threadIdx.x;
-  static_assert(kMaxSplits <= 256, "a thread per share");
-  const bool mine = (int32_t)t < rg.active;
-  const float ref = mine ? w[t * kShare<D> + kCols * D + c] : kNever;
-  const float sum = mine ? w[t * kShare<D> + kCols * D + kCols + c] : 0;
-  const float top = wave_max(ref);
-  if (t % 64 == 0) red[t / 64] = top;
+// The segments of one column of an item and head, joined, where there are more
+// than one: a workgroup per item and column, and head.  The segments' weights
+// first, then D threads add up their O, TH / D groups of them every so many segments.
+template <int NB, int TH, typename T>
+__global__ __launch_bounds__(TH) void kv4_attn_join_kernel(AttnArgs a, uint32_t tile_cols) {
+  constexpr int D = NB * 32, G = TH / D;
+  const uint32_t item = blockIdx.x / tile_cols, c = blockIdx.x % tile_cols, head = blockIdx.y;
+  const Item t = item_of(a, item);
+  if (t.col0 + c >= t.cols || t.steps == 0) return;
+  const uint32_t share = kv4_const(a.starts);
+  const uint32_t from = kv4_const(a.starts + 1 + item) + head * ((uint32_t)t.steps + kOverhead) + kOverhead;
+  const uint32_t w0 = from / share, count = (from + (uint32_t)t.steps - 1) / share - w0 + 1;
+  if (count == 1) return;
+  __shared__ float weight[kMaxGroups], sums[G][D], red[32];
+  // the workgroup that began the head has it in its place 1, the others in their place 0
+  const float *w = a.work + 2 * (size_t)w0 * kShare<D>;
+  const uint32_t th = threadIdx.x;
+  auto part = [&](uint32_t n) { return w + (2 * (size_t)n + (n == 0)) * kShare<D>; };
+  float top = kNever, sum = 0;
+  for (uint32_t n = th; n < count; n += TH) top = __builtin_fmaxf(top, weight[n] = part(n)[kCols * D + c]);
+  top = wave_max(top);
+  if (th % 64 == 0) red[th / 64] = top;
   __syncthreads();
-  const float f = __builtin_amdgcn_exp2f(ref - __builtin_fmaxf(__builtin_fmaxf(red[0], red[1]),
-                                                               __builtin_fmaxf(red[2], red[3])));
-  const float all = wave_sum(sum * f);
-  if (t % 64 == 0) red[4 + t / 64] = all;
-  if (mine) weight[t] = f;
+#pragma unroll
+  for (int n = 0; n < TH / 64; ++n) top = __builtin_fmaxf(top, red[n]);
+  for (uint32_t n = th; n < count; n += TH) {
+    const float f = __builtin_amdgcn_exp2f(weight[n] - top);
+    sum = __builtin_fmaf(part(n)[kCols * D + kCols + c], f, sum);
+    weight[n] = f;
+  }
+  sum = wave_sum(sum);
+  if (th % 64 == 0) red[16 + th / 64] = sum;
   __syncthreads();
-  const uint32_t grp = t / D, d = t % D;
+  const uint32_t grp = th / D, d = th % D;
   if (grp < G) {
     float o = 0;
 #pragma unroll 8
-    for (int32_t n = grp; n < rg.active; n += G) o = __builtin_fmaf(w[n * kShare<D> + c * D + d], weight[n], o);
-    part[grp][d] = o;
+    for (uint32_t n = grp; n < count; n += G)
+      o = __builtin_fmaf(part(n)[c * D + d], weight[n], o);
+    sums[grp][d] = o;
   }
   __syncthreads();
-  if (t < D) {
-    float o = 0;
+  if (th < D) {
+    float o = 0, l = 0;
 #pragma unroll
-    for (int g = 0; g < G; ++g) o += part[g][t];
-    const float l = (red[4] + red[5]) + (red[6] + red[7]);
-    const uint32_t orow = s.row0 + (col0 + c) / a.group, oh = head * a.group + (col0 + c) % a.group;
-    put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + t, l == 0 ? 0.0f : o / l);
+    for (int n = 0; n < G; ++n) o += sums[n][th];
+#pragma unroll
+    for (int n = 0; n < TH / 64; ++n) l += red[16 + n];
+    const uint32_t orow = t.s.row0 + (t.col0 + c) / a.group, oh = head * a.group + (t.col0 + c) % a.group;
+    put<T>(static_cast<T *>(a.out) + (size_t)orow * a.ldo + (size_t)oh * D + th, l == 0 ? 0.0f : o / l);
   }
 }
 
 struct Plan {
-  uint32_t tiles, splits, min_steps;
-  size_t share;  // bytes of one split of one tile
+  uint32_t tiles, groups;  // groups: workgroups that share the steps, 0: one per tile and head
+  size_t part;             // bytes of a partial result
+  size_t starts;           // bytes of the items' starts
+  size_t bytes() const { return groups ? groups * 2 * part + starts : 0; }
 };
-// How many workgroups may share the keys of a tile, and the fewest steps of a
-// share: two workgroups per CU if every sequence had len_max keys, but shares
-// of no more than 64 steps (a batch's lengths may differ; the long ones must
-// not be what the call waits for) and of no less than 8 (two per wave).
-Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, uint32_t cus) {
-  Plan p;
+// A cache of up to 16 steps (four per wave) stays with one workgroup per tile and
+// head.  Longer ones are dealt out over as many workgroups as are resident at once.
+Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype, uint32_t cus) {
+  Plan p = {};
   const uint64_t reach = (uint64_t)b->max_pages * c->page;
   const uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
-  const uint64_t cols = (uint64_t)b->rows * (nh / c->nkv);
-  p.tiles = (uint32_t)((cols + kCols - 1) / kCols);
-  p.share = (size_t)kCols * (c->d + 2) * 4;
-  const uint64_t groups = (uint64_t)p.tiles * c->nkv * b->b, steps = (len + kKeys - 1) / kKeys;
-  uint64_t per = groups * steps / (2 * cus);
-  per = per > 64 ? 64 : per < 8 ? 8 : per;
-  uint64_t want = (steps + per - 1) / per;
-  if (groups >= 8ull * cus) want = 1;
-  p.min_steps = (uint32_t)per;
-  p.splits = (uint32_t)(want > kMaxSplits ? kMaxSplits : want < 1 ? 1 : want);
+  p.tiles = (uint32_t)(((uint64_t)b->rows * (nh / c->nkv) + kCols - 1) / kCols);
+  p.part = (size_t)kCols * (c->d + 2) * 4;
+  const uint64_t items = (uint64_t)p.tiles * b->b;
+  p.starts = (size_t)(items + 1) * 4;
+  if ((len + kKeys - 1) / kKeys <= 16) return p;
+  // (the row's places are counted in 32 bits)
+  if (items * c->nkv * ((reach + kKeys - 1) / kKeys + kOverhead + 1) > 0x40000000u) return p;
+  p.groups = resident(c->d, dtype == MADI_F32) * cus;
+  p.groups = p.groups < kMaxGroups ? p.groups : kMaxGroups;
   return p;
 }
 
 template <int NB, typename T>
-void launch(const AttnArgs &a, uint32_t tiles, uint32_t b) {
-  kv4_attn_kernel<NB, 4, T><<<dim3(tiles * a.splits, a.kv.nkv, b), 256, 0, stream()>>>(a);
+void launch(const AttnArgs &a, uint32_t groups, uint32_t cus) {
+  if (!a.shared) {
+    kv4_attn_kernel<NB, 8, T><<<a.items * a.kv.nkv, 512, 0, stream()>>>(a);
+    return;
+  }
+  kv4_attn_kernel<NB, 4, T><<<groups, 256, 0, stream()>>>(a);
   const uint64_t cols = (uint64_t)a.kv.rows * a.group;
   const uint32_t tile_cols = cols < kCols ? (uint32_t)cols : kCols;
-  if (a.splits > 1)
-    kv4_attn_join_kernel<NB, T><<<dim3(tiles * tile_cols, a.kv.nkv, b), 256, 0, stream()>>>(a, tiles, tile_cols);
+  const dim3 grid(a.items * tile_cols, a.kv.nkv);
+  // few columns are of long caches, many segments each; of many most have one
+  if ((uint64_t)grid.x * grid.y <= 2 * cus)
+    kv4_attn_join_kernel<NB, 1024, T><<<grid, 1024, 0, stream()>>>(a, tile_cols);
+  else
+    kv4_attn_join_kernel<NB, 256, T><<<grid, 256, 0, stream()>>>(a, tile_cols);
 }
 
 }  // namespace
@@ -641,8 +843,8 @@ void launch(const AttnArgs &a, uint32_t tiles, uint32_t b) {
 extern "C" size_t madi_kv4_attn_bytes(const madi_kv4 *cache, const madi_kv4_batch *batch, uint32_t nh) {
   Kv4Args a;
   if (kv4_args("madi_kv4_attn_bytes", cache, batch, &a) || nh == 0 || nh % cache->nkv) return 0;
-  const Plan p = plan_of(cache, batch, nh, initialized() ? (uint32_t)cu_count() : 256);
-  return p.splits > 1 ? (size_t)p.tiles * cache->nkv * batch->b * p.splits * p.share : 0;
+  const Plan p = plan_of(cache, batch, nh, MADI_F16, initialized() ? (uint32_t)cu_count() : 256);
+  return p.bytes();
 }
 
 extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, const madi_kv4_batch *batch,
@@ -671,16 +873,17 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
     return fail(MADI_ERR_SHAPE, "%s: %u rows of a sequence in one call", what, batch->rows);
   if (!initialized()) return fail(MADI_ERR_NOT_INIT, "%s: madi_init has not succeeded", what);
   if (batch->m == 0 || batch->b == 0 || batch->rows == 0) return MADI_OK;
-  Plan p = plan_of(cache, batch, nh, (uint32_t)cu_count());
-  // as many splits as the workspace holds
-  const size_t each = (size_t)p.tiles * cache->nkv * batch->b * p.share;
-  if ((size_t)p.splits * each > wb) p.splits = wb / each > 1 ? (uint32_t)(wb / each) : 1;
-  if ((uint64_t)p.tiles * p.splits > 0x7fffffffu)
-    return fail(MADI_ERR_SHAPE, "%s: %u rows of a sequence in one call", what, batch->rows);
+  Plan p = plan_of(cache, batch, nh, dtype, (uint32_t)cu_count());
+  // as many workgroups as the workspace has places for
+  if (p.bytes() > wb) p.groups = wb > p.starts ? (uint32_t)((wb - p.starts) / (2 * p.part)) : 0;
+  if (p.groups < 2) p.groups = 0;
+  const uint64_t items = (uint64_t)p.tiles * batch->b;
+  if (items * cache->nkv * kCols > 0x7fffffffu)
+    return fail(MADI_ERR_SHAPE, "%s: %u rows of %u sequences in one call", what, batch->rows, batch->b);
   if (int rc = deferred_before_read(q, qb)) return rc;
   if (int rc = deferred_before_read(cache->data, cb)) return rc;
   if (int rc = deferred_before_write(out, ob)) return rc;
-  if (p.splits > 1)
+  if (p.groups)
     if (int rc = deferred_before_write(batch->work, wb)) return rc;
   a.q = q;
   a.out = out;
@@ -690,15 +893,18 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
   a.group = nh / cache->nkv;
   a.window = window;
   a.causal = (uint32_t)causal;
-  a.splits = p.splits;
-  a.min_steps = p.min_steps;
+  a.tiles = p.tiles;
+  a.items = (uint32_t)items;
+  a.shared = p.groups != 0;
+  a.starts = reinterpret_cast<uint32_t *>(a.work + p.groups * 2 * (p.part / 4));
   a.scale = scale;
   const bool f = dtype == MADI_F32;
+  const uint32_t cus = (uint32_t)cu_count();
   switch (cache->d) {
-  case 64: f ? launch<2, float>(a, p.tiles, batch->b) : launch<2, f16>(a, p.tiles, batch->b); break;
-  case 96: f ? launch<3, float>(a, p.tiles, batch->b) : launch<3, f16>(a, p.tiles, batch->b); break;
-  case 128: f ? launch<4, float>(a, p.tiles, batch->b) : launch<4, f16>(a, p.tiles, batch->b); break;
-  default: f ? launch<8, float>(a, p.tiles, batch->b) : launch<8, f16>(a, p.tiles, batch->b); break;
+  case 64: f ? launch<2, float>(a, p.groups, cus) : launch<2, f16>(a, p.groups, cus); break;
+  case 96: f ? launch<3, float>(a, p.groups, cus) : launch<3, f16>(a, p.groups, cus); break;
+  case 128: f ? launch<4, float>(a, p.groups, cus) : launch<4, f16>(a, p.groups, cus); break;
+  default: f ? launch<8, float>(a, p.groups, cus) : launch<8, f16>(a, p.groups, cus); break;
   }
   return check_launch(what);
 }
