@@ -50,6 +50,10 @@ constexpr size_t kShare = kCols * (D + 2);
 // the low parts) and by LDS (the ring).
 constexpr uint32_t resident(uint32_t d, bool f32) { return d == 256 ? 2 : f32 && d == 128 ? 3 : 4; }
 
+// Waves of a workgroup that has a tile and head for itself: as many as fit a CU's
+// registers.
+constexpr uint32_t waves_alone(uint32_t d, bool f32) { return 4 * resident(d, f32) > 12 ? 16 : 8; }
+
 struct AttnArgs {
   Kv4Args kv;
   const void *q;
@@ -127,10 +131,14 @@ struct Step {
   bool there[2];
 };
 
-// Pages of the tiles at key and key + 16 (none past the end).
-__device__ inline void find_pages(uint32_t (&page)[2], const Kv4Args &a, uint32_t seq, int32_t key, int32_t len) {
+// Page numbers of the tiles at key and key + 16, within the table's reach (the
+// first ones are asked for beside the sequence's length, not after it).
+__device__ inline void find_pages(uint32_t (&page)[2], const Kv4Args &a, uint32_t seq, uint32_t key) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) page[i] = key + 16 * i < len ? kv4_page(a, seq, key + 16 * i) : 0xffffffffu;
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t n = (key + 16 * i) >> a.shift;
+    page[i] = kv4_const(a.table + (size_t)seq * a.max_pages + (n < a.max_pages ? n : 0));
+  }
 }
 
 // A wave's ring of steps in LDS.  Every lane reads back what it loaded itself,
@@ -139,7 +147,6 @@ __device__ inline void find_pages(uint32_t (&page)[2], const Kv4Args &a, uint32_
 // per lane; a piece's 64 lanes lie side by side.
 template <int NB>
 struct Ring {
-  static constexpr int kDepth = NB == 2 ? 4 : 2;
   static constexpr int kWide = NB / 4, kNarrow = NB % 4;  // pieces of NB words
   static constexpr int kScales = Step<NB>::kScaleWords;
   static constexpr int kTile = 256 * (2 * NB + kScales), kBytes = 2 * kTile;
@@ -169,15 +176,15 @@ __device__ inline void read_pieces(uint32_t (&w)[NB], const uint8_t *from, uint3
 // Starts the loads of the step at `key` into the ring's slot at LDS address
 // `to`; returns which tiles have a page (bits 0 and 1).
 template <int NB>
-__device__ inline uint32_t fetch(const Kv4Args &a, const uint32_t (&pages)[2], uint32_t head, int32_t key, uint32_t lane,
-                                 uint32_t to) {
+__device__ inline uint32_t fetch(const Kv4Args &a, const uint32_t (&pages)[2], uint32_t head, int32_t key, int32_t len,
+                                 uint32_t lane, uint32_t to) {
   constexpr uint32_t D = NB * 32;
   const uint32_t r = lane & 15, g = lane >> 4;
   uint32_t there = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    // a tile without a page: any valid one stands in
-    const bool ok = pages[i] < a.n_pages;
+    // a tile past the end or without a page: any valid one stands in
+    const bool ok = key + 16 * i < len && pages[i] < a.n_pages;
     there |= ok ? 1u << i : 0;
     const uint32_t off = (uint32_t)(key + 16 * i) & ((1u << a.shift) - 1);
     const uint8_t *blk = kv4_block(a, ok ? pages[i] : 0, head, D);
@@ -223,60 +230,47 @@ struct Query {
   float fac;  // score from the product: scale * log2(e) / 2^k
 };
 
-template <typename T>
-__device__ inline void load8f(const T *p, float (&x)[8]);
-template <>
-__device__ inline void load8f<float>(const float *p, float (&x)[8]) {
-  const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
+// q of the lane's column as it lies in memory: the 8 elements of each block that
+// slot group g multiplies.
+template <int NB, typename T>
+struct RawQuery {
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  vec8 x[NB];
+  __device__ inline RawQuery(const T *q) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-}
-template <>
-__device__ inline void load8f<f16>(const f16 *p, float (&x)[8]) {
-  const f16x8 a = *reinterpret_cast<const f16x8 *>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
-}
-
-// q of the lane's column (the 8 elements of each block that slot group g
-// multiplies).  An f32 row is brought to [2^10, 2^11) by a power of two 2^k, so
+    for (int b = 0; b < NB; ++b) x[b] = *reinterpret_cast<const vec8 __attribute__((aligned(16))) *>(q + 32 * b);
+  }
+};
+// As operands.  An f32 row is brought to [2^10, 2^11) by a power of two 2^k, so
 // that its low parts lose nothing that counts.
 template <int NB, int P, typename T>
-__device__ inline void load_query(Query<NB, P> &Q, const T *q, bool there, uint32_t g, float scale) {
-  float x[NB][8], top = 0;
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    if (there) {
-      load8f<T>(q + 32 * b + 8 * g, x[b]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[b][e] = 0;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, __builtin_fabsf(x[b][e]));
-  }
+__device__ inline void make_query(Query<NB, P> &Q, const RawQuery<NB, T> &raw, bool there, float scale) {
   int k = 0;
   if (P == 2) {
+    float top = 0;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, __builtin_fabsf((float)raw.x[b][e]));
     top = max_across(top);
     k = top > 0 && top < __builtin_inff() ? 11 - __builtin_amdgcn_frexp_expf(top) : 0;
     k = k < -100 ? -100 : k > 100 ? 100 : k;
   }
   // (never 0, so that it leaves the - infinity of a key not seen what it is)
   Q.fac = __builtin_fmaxf(__builtin_ldexpf(__builtin_fabsf(scale) * 1.4426950408889634f, -k), 1e-37f);
-  const float sign = scale < 0 ? -1.0f : 1.0f;
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      f16x8 h;
+  for (int b = 0; b < NB; ++b) {
+    if constexpr (P == 1) {
+      Q.q[b][0] = there ? (scale < 0 ? -raw.x[b] : raw.x[b]) : (f16x8){0, 0, 0, 0, 0, 0, 0, 0};
+    } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (p == 0) x[b][e] = __builtin_ldexpf(x[b][e], k) * sign;
-        h[e] = (f16)x[b][e];
-        x[b][e] -= (float)h[e];
+        const float x = there ? __builtin_ldexpf(scale < 0 ? -raw.x[b][e] : raw.x[b][e], k) : 0.0f;
+        Q.q[b][0][e] = (f16)x;
+        Q.q[b][1][e] = (f16)(x - (float)Q.q[b][0][e]);
       }
-      Q.q[b][p] = h;
     }
+  }
 }
 
 // Nibbles 0 and 4 (HIGH: 1 and 5) of w as the codes' values: the f16 numbers
@@ -512,27 +506,19 @@ __device__ inline void put<float>(float *out, float v) { *out = v; }
 template <>
 __device__ inline void put<f16>(f16 *out, float v) { *out = (f16)v; }
 
-// Sum over the workgroup's threads before the caller, and over all.
-template <int W>
-__device__ inline uint32_t scan(uint32_t v, uint32_t &all, uint32_t *lds) {
-  uint32_t x = v;
-  const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-  for (uint32_t n = 1; n < 64; n *= 2) {
-    const uint32_t y = __shfl_up(x, n);
-    x += lane >= n ? y : 0;
-  }
-  __syncthreads();
-  if (lane == 63) lds[threadIdx.x / 64] = x;
-  __syncthreads();
-  all = 0;
-  uint32_t before = 0;
-#pragma unroll
-  for (uint32_t w = 0; w < W; ++w) {
-    before += w < threadIdx.x / 64 ? lds[w] : 0;
-    all += lds[w];
-  }
-  return before + x - v;
+// Sum over the wave's lanes up to and with the caller's.
+template <int CTRL, int ROWS = 0xf>
+__device__ inline uint32_t shifted(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ inline uint32_t wave_scan(uint32_t v) {
+  v += shifted<0x111>(v);  // row_shr 1, 2, 4, 8
+  v += shifted<0x112>(v);
+  v += shifted<0x114>(v);
+  v += shifted<0x118>(v);
+  v += shifted<0x142, 0xa>(v);  // row_bcast 15: rows 0 and 2 into 1 and 3
+  v += shifted<0x143, 0xc>(v);  // row_bcast 31: the lower half into the upper
+  return v;
 }
 
 // W waves on the same 16 columns, wave w taking steps w, w + W, .. of the
@@ -549,14 +535,13 @@ template <int NB, int W, typename T>
 __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4_attn_kernel(AttnArgs a) {
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
   constexpr int D = NB * 32;
-  constexpr int R = Ring<NB>::kDepth;
+  constexpr int R = NB == 2 && W == 4 ? 4 : 2;  // as deep as LDS lets the waves be
   struct Results {
-    float ref[W][kCols], sum[W][kCols], o[W][kCols][D + 4];
+    float ref[kCols][W], sum[kCols][W], o[W][kCols][D + 4];
   };
   constexpr size_t kLds = sizeof(Results) > (size_t)W * R * Ring<NB>::kBytes ? sizeof(Results)
                                                                              : (size_t)W * R * Ring<NB>::kBytes;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
-  uint32_t *found = reinterpret_cast<uint32_t *>(lds);  // before the ring is used
   Results &res = *reinterpret_cast<Results *>(lds);
 
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -568,40 +553,39 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
   // The workgroup's part [at, end) of the row, from place `in` of item `item`
   uint32_t item, in, left;
   if (a.shared) {
-    // the length of all items, then the one that holds place `from` (up to as
-    // many items as threads, both from one scan)
-    uint32_t total = 0, all, len = 0, start = 0;
-    for (uint32_t i = 0; i < a.items; i += 64 * W) {
-      const uint32_t n = i + threadIdx.x;
-      len = n < a.items ? item_length(a, item_of(a, n)) : 0;
-      start = total + scan<W>(len, all, found + 2);
-      total += all;
+    // The length of all items, then the one that holds place `from`; every wave
+    // by itself, 64 items at a time (up to 64, both from one scan).
+    uint32_t total = 0, upto = 0, len = 0;
+    for (uint32_t i = 0; i < a.items; i += 64) {
+      len = i + lane < a.items ? item_length(a, item_of(a, i + lane)) : 0;
+      upto = wave_scan(len);
+      total += __builtin_amdgcn_readlane(upto, 63);
     }
     uint32_t share = (total + gridDim.x - 1) / gridDim.x;
     share = share > kOverhead + W ? share : kOverhead + W;
     const uint32_t from = blockIdx.x * share;  // below total + share
-    if (threadIdx.x == 0) found[0] = a.items;
-    __syncthreads();
-    uint32_t base = 0;
-    for (uint32_t i = 0; i < a.items; i += 64 * W) {
-      const uint32_t n = i + threadIdx.x;
-      if (a.items > 64 * W) {
-        len = n < a.items ? item_length(a, item_of(a, n)) : 0;
-        start = base + scan<W>(len, all, found + 2);
-        base += all;
+    item = a.items;
+    in = 0;
+    for (uint32_t i = 0, base = 0; i < a.items; i += 64) {
+      if (a.items > 64) {
+        len = i + lane < a.items ? item_length(a, item_of(a, i + lane)) : 0;
+        upto = wave_scan(len);
       }
-      if (from >= start && from - start < len) {
-        found[0] = n;
-        found[1] = from - start;
+      const uint32_t start = base + upto - len;
+      const uint64_t here = __ballot(from >= start && from - start < len);
+      if (here) {
+        const int n = __builtin_ctzll(here);
+        item = i + n;
+        in = from - __builtin_amdgcn_readlane(start, n);
       }
-      if (blockIdx.x == 0 && n < a.items) a.starts[1 + n] = start;
+      if (blockIdx.x == 0 && wave == 0 && i + lane < a.items) a.starts[1 + i + lane] = start;
+      base += __builtin_amdgcn_readlane(upto, 63);
+      if (here && blockIdx.x != 0) break;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) a.starts[0] = share;
-    __syncthreads();
-    item = __builtin_amdgcn_readfirstlane(found[0]);
-    in = __builtin_amdgcn_readfirstlane(found[1]);
+    item = __builtin_amdgcn_readfirstlane(item);
+    in = __builtin_amdgcn_readfirstlane(in);
     left = share;
-    __syncthreads();
   } else {
     item = blockIdx.x / a.kv.nkv;
     in = blockIdx.x % a.kv.nkv;  // of heads
@@ -656,23 +640,25 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
       int32_t at = begin + (int32_t)wave, issued = at;
       uint32_t slot_in = 0, there_in = 0;  // next slot to load; which tiles of the ring's slots have pages
       uint32_t pages[2];
-      find_pages(pages, a.kv, t.seq, (t.first + issued) * kKeys, issued < end ? s.len : 0);
+      find_pages(pages, a.kv, t.seq, (t.first + issued) * kKeys);
       auto issue = [&]() {
         if (issued < end) {
-          const uint32_t ok = fetch<NB>(a.kv, pages, head, (t.first + issued) * kKeys, lane,
+          const uint32_t ok = fetch<NB>(a.kv, pages, head, (t.first + issued) * kKeys, s.len, lane,
                                         ring_at + slot_in * Ring<NB>::kBytes);
           there_in = (there_in & ~(3u << (2 * slot_in))) | ok << (2 * slot_in);
           slot_in = slot_in + 1 == R ? 0 : slot_in + 1;
           issued += W;
-          find_pages(pages, a.kv, t.seq, (t.first + issued) * kKeys, issued < end ? s.len : 0);
+          find_pages(pages, a.kv, t.seq, (t.first + issued) * kKeys);
         }
       };
+      // (the queries are asked for first: theirs is the shorter way)
+      const RawQuery<NB, T> raw(static_cast<const T *>(a.q) + (size_t)(s.row0 + row) * a.ldq +
+                                (size_t)(head * a.group + sub) * D + 8 * g);
 #pragma unroll 1
       for (int n = 0; n < R - 1; ++n) issue();
 
       Query<NB, P> Q;
-      load_query<NB, P, T>(Q, static_cast<const T *>(a.q) + (size_t)(s.row0 + row) * a.ldq +
-                                  (size_t)(head * a.group + sub) * D, mine, g, a.scale);
+      make_query<NB, P, T>(Q, raw, mine, a.scale);
       Acc<NB> A;
       A.ref = kNever;
       A.sum = 0;
@@ -703,30 +689,28 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
         at += W;
       }
       A.sum = sum_across(A.sum);
-      const float up = 1 / A.down;  // a power of two
-
-      // the waves' results: a common reference, then sums over the waves
+          // the waves' results: brought to a common reference, then added up
       __syncthreads();
-      if (g == 0) {
-        res.ref[wave][r] = A.ref;
-        res.sum[wave][r] = A.sum;
-      }
+      if (g == 0) res.ref[r][wave] = A.ref;
+      __syncthreads();
+      float ref = kNever;
+#pragma unroll
+      for (int w = 0; w < W; ++w) ref = __builtin_fmaxf(ref, res.ref[r][w]);
+      const float f = __builtin_amdgcn_exp2f(A.ref - ref), fo = f / A.down;  // (a power of two)
+      if (g == 0) res.sum[r][wave] = A.sum * f;
       if (mine)
 #pragma unroll
-        for (int n = 0; n < 2 * NB; ++n) *reinterpret_cast<f32x4 *>(&res.o[wave][r][16 * n + 4 * g]) = A.o[n] * up;
+        for (int n = 0; n < 2 * NB; ++n) *reinterpret_cast<f32x4 *>(&res.o[wave][r][16 * n + 4 * g]) = A.o[n] * fo;
       __syncthreads();
       const uint32_t ncols = t.cols - t.col0 < kCols ? t.cols - t.col0 : kCols;
       float *part = a.work + (2 * (size_t)blockIdx.x + (begin == 0)) * kShare<D>;
       for (uint32_t i = threadIdx.x; i < ncols * D; i += 64 * W) {
         const uint32_t c = i / D, d = i % D;
-        float ref = kNever, o = 0, sum = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) ref = __builtin_fmaxf(ref, res.ref[w][c]);
+        float o = 0, sum = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const float f = __builtin_amdgcn_exp2f(res.ref[w][c] - ref);
-          sum = __builtin_fmaf(res.sum[w][c], f, sum);
-          o = __builtin_fmaf(res.o[w][c][d], f, o);
+          sum += res.sum[c][w];
+          o += res.o[w][c][d];
         }
         if (whole_head) {
           const uint32_t orow = s.row0 + (t.col0 + c) / a.group, oh = head * a.group + (t.col0 + c) % a.group;
@@ -734,6 +718,9 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
         } else {
           part[i] = o;
           if (d == 0) {
+            ref = kNever;
+#pragma unroll
+            for (int w = 0; w < W; ++w) ref = __builtin_fmaxf(ref, res.ref[c][w]);
             part[kCols * D + c] = ref;
             part[kCols * D + kCols + c] = sum;
           }
@@ -799,21 +786,23 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(AttnArgs a, uint32_t 
 
 struct Plan {
   uint32_t tiles, groups;  // groups: workgroups that share the steps, 0: one per tile and head
+  bool few;                // steps, for which four waves do
   size_t part;             // bytes of a partial result
   size_t starts;           // bytes of the items' starts
   size_t bytes() const { return groups ? groups * 2 * part + starts : 0; }
 };
-// A cache of up to 16 steps (four per wave) stays with one workgroup per tile and
-// head.  Longer ones are dealt out over as many workgroups as are resident at once.
-Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype, uint32_t cus) {
+// A cache of up to four steps per wave stays with one workgroup per tile and head.  Longer ones are dealt out over as many workgroups as are resident at once.
+Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype, uint32_t window, uint32_t cus) {
   Plan p = {};
   const uint64_t reach = (uint64_t)b->max_pages * c->page;
-  const uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
+  uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
+  if (window && (uint64_t)window + b->rows + kKeys < len) len = (uint64_t)window + b->rows + kKeys;
   p.tiles = (uint32_t)(((uint64_t)b->rows * (nh / c->nkv) + kCols - 1) / kCols);
   p.part = (size_t)kCols * (c->d + 2) * 4;
   const uint64_t items = (uint64_t)p.tiles * b->b;
   p.starts = (size_t)(items + 1) * 4;
-  if ((len + kKeys - 1) / kKeys <= 16) return p;
+  p.few = (len + kKeys - 1) / kKeys <= 8;
+  if ((len + kKeys - 1) / kKeys <= 4 * waves_alone(c->d, dtype == MADI_F32)) return p;
   // (the row's places are counted in 32 bits)
   if (items * c->nkv * ((reach + kKeys - 1) / kKeys + kOverhead + 1) > 0x40000000u) return p;
   p.groups = resident(c->d, dtype == MADI_F32) * cus;
@@ -822,9 +811,11 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
 }
 
 template <int NB, typename T>
-void launch(const AttnArgs &a, uint32_t groups, uint32_t cus) {
+void launch(const AttnArgs &a, uint32_t groups, bool few, uint32_t cus) {
   if (!a.shared) {
-    kv4_attn_kernel<NB, 8, T><<<a.items * a.kv.nkv, 512, 0, stream()>>>(a);
+    constexpr int W = waves_alone(NB * 32, sizeof(T) == 4);
+    if (few) kv4_attn_kernel<NB, 4, T><<<a.items * a.kv.nkv, 256, 0, stream()>>>(a);
+    else kv4_attn_kernel<NB, W, T><<<a.items * a.kv.nkv, 64 * W, 0, stream()>>>(a);
     return;
   }
   kv4_attn_kernel<NB, 4, T><<<groups, 256, 0, stream()>>>(a);
@@ -843,7 +834,7 @@ void launch(const AttnArgs &a, uint32_t groups, uint32_t cus) {
 extern "C" size_t madi_kv4_attn_bytes(const madi_kv4 *cache, const madi_kv4_batch *batch, uint32_t nh) {
   Kv4Args a;
   if (kv4_args("madi_kv4_attn_bytes", cache, batch, &a) || nh == 0 || nh % cache->nkv) return 0;
-  const Plan p = plan_of(cache, batch, nh, MADI_F16, initialized() ? (uint32_t)cu_count() : 256);
+  const Plan p = plan_of(cache, batch, nh, MADI_F16, 0, initialized() ? (uint32_t)cu_count() : 256);
   return p.bytes();
 }
 
@@ -873,7 +864,7 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
     return fail(MADI_ERR_SHAPE, "%s: %u rows of a sequence in one call", what, batch->rows);
   if (!initialized()) return fail(MADI_ERR_NOT_INIT, "%s: madi_init has not succeeded", what);
   if (batch->m == 0 || batch->b == 0 || batch->rows == 0) return MADI_OK;
-  Plan p = plan_of(cache, batch, nh, dtype, (uint32_t)cu_count());
+  Plan p = plan_of(cache, batch, nh, dtype, window, (uint32_t)cu_count());
   // as many workgroups as the workspace has places for
   if (p.bytes() > wb) p.groups = wb > p.starts ? (uint32_t)((wb - p.starts) / (2 * p.part)) : 0;
   if (p.groups < 2) p.groups = 0;
@@ -901,10 +892,10 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
   const bool f = dtype == MADI_F32;
   const uint32_t cus = (uint32_t)cu_count();
   switch (cache->d) {
-  case 64: f ? launch<2, float>(a, p.groups, cus) : launch<2, f16>(a, p.groups, cus); break;
-  case 96: f ? launch<3, float>(a, p.groups, cus) : launch<3, f16>(a, p.groups, cus); break;
-  case 128: f ? launch<4, float>(a, p.groups, cus) : launch<4, f16>(a, p.groups, cus); break;
-  default: f ? launch<8, float>(a, p.groups, cus) : launch<8, f16>(a, p.groups, cus); break;
+  case 64: f ? launch<2, float>(a, p.groups, p.few, cus) : launch<2, f16>(a, p.groups, p.few, cus); break;
+  case 96: f ? launch<3, float>(a, p.groups, p.few, cus) : launch<3, f16>(a, p.groups, p.few, cus); break;
+  case 128: f ? launch<4, float>(a, p.groups, p.few, cus) : launch<4, f16>(a, p.groups, p.few, cus); break;
+  default: f ? launch<8, float>(a, p.groups, p.few, cus) : launch<8, f16>(a, p.groups, p.few, cus); break;
   }
   return check_launch(what);
 }
