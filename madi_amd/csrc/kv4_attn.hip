@@ -31,6 +31,11 @@ namespace {
 
 constexpr int kCols = 16;  // columns of a wave (MFMA columns)
 constexpr int kKeys = 32;  // keys of a step
+// A prompt's workgroup: waves, tiles of 16 columns per wave (two where the
+// registers allow it), keys in a buffer (two buffers fit LDS).
+constexpr int kPromptWaves = 8;
+constexpr int prompt_tiles(int d, bool f32) { return d < 128 || (d == 128 && !f32) ? 2 : 1; }
+constexpr int prompt_keys(int d) { return d == 256 ? 32 : 64; }
 constexpr float kNever = -1e30f;  // reference before any key was seen
 // P is 2^(x - M) with M at first the largest x - 7, raised when an x passes M
 // by 14: P at most 2^14, P s 2^-e at most 2^15 (f16 holds 2^16), and what
@@ -473,16 +478,17 @@ struct Item {
   int32_t first, steps;
   bool none;                 // past the sequence's columns
 };
+template <uint32_t COLS = kCols>
 __device__ inline Item item_of(const AttnArgs &a, uint32_t item) {
   Item t;
   t.seq = a.tiles == 1 ? item : item / a.tiles;
-  t.col0 = (item - t.seq * a.tiles) * kCols;
+  t.col0 = (item - t.seq * a.tiles) * COLS;
   t.s = kv4_seq(a.kv, t.seq);
   t.cols = t.s.nrows * a.group;
   t.none = t.col0 >= t.cols;
   int32_t lo = 0, hi = t.s.len;
   if (a.causal) {
-    const uint32_t last = (t.col0 + kCols < t.cols ? t.col0 + kCols : t.cols) - 1;
+    const uint32_t last = (t.col0 + COLS < t.cols ? t.col0 + COLS : t.cols) - 1;
     const int32_t p0 = t.s.pos0 + (int32_t)(t.col0 / a.group), p1 = t.s.pos0 + (int32_t)(last / a.group);
     hi = p1 + 1 < hi ? p1 + 1 : hi;
     if (a.window && p0 >= (int32_t)a.window) lo = p0 - (int32_t)a.window + 1;
@@ -784,9 +790,352 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(AttnArgs a, uint32_t 
   }
 }
 
+// ---------------------------------------------------------------- prompts
+// Many columns: NW waves with two tiles of 16 columns each walk the same keys,
+// KC at a time, and share what turning the words into f16 operands costs: the
+// next KC keys' operands go to LDS while these are multiplied (two buffers, one
+// barrier per KC keys), the words of the ones after that are on their way in
+// registers.  The operands lie in LDS as the MFMAs read them, 16 bytes per lane.
+//   K as its codes (the block sums get their scales, f16 in LDS, afterwards);
+//   V as (n - 8) s in two f16, which hold all of its 15 bits: rounded to one
+//     it would add an error like P's own rounding, and so would K.
+// For 64 keys and 16 columns at d 128 that is 48 MFMAs (768 cycles) and about 200
+// vector instructions (800 cycles), against 64 scores per lane group.
+template <int NB, int KC>
+struct Buffer {
+  static constexpr int kTiles = KC / 16;
+  u32x4 k[kTiles][NB][64];           // [lane]: key lane % 16, elements 8 (lane / 16) ..
+  u32x4 v[2][KC / 32][2 * NB][64];   // [high, low][pair of tiles][16 elements][lane]
+  float ks[kTiles][NB][16];          // [key], times the scores' factor
+  uint32_t there[kTiles];
+};
+
+// A wave's share of the words of KC keys: of a tile of 16 keys, wave `part` of
+// its kPer has blocks part, part + kPer, ..
+template <int NB, int KC, int NW>
+struct Words {
+  static constexpr int kPer = NW / (KC / 16);
+  static constexpr int kBlocks = (NB + kPer - 1) / kPer;
+  uint32_t k[kBlocks], v[kBlocks], s[kBlocks][2], ks, there;
+  static __device__ inline uint32_t block(int i, uint32_t part) {
+    const uint32_t b = part + i * kPer;
+    return NB % kPer == 0 || b < NB ? b : NB - 1;  // (the last one twice)
+  }
+  __device__ inline void fetch(const Kv4Args &a, uint32_t page, uint32_t head, int32_t key, int32_t len, uint32_t part,
+                               uint32_t lane) {
+    constexpr uint32_t D = NB * 32;
+    const uint32_t r = lane & 15, g = lane >> 4;
+    there = key < len && page < a.n_pages;
+    page = there ? page : 0;
+    const uint32_t off = (uint32_t)key & ((1u << a.shift) - 1);
+    const uint8_t *blk = kv4_block(a, page, head, D);
+    const uint8_t *kp = blk + (size_t)off * (D / 2), *vp = kp + ((size_t)(D / 2) << a.shift);
+    const uint8_t *sp = blk + ((size_t)D << a.shift) + (size_t)off * (D / 8) + g * (D / 2);
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      const uint32_t b = block(i, part);
+      k[i] = *reinterpret_cast<const uint32_t *>(kp + 4 * b + r * (D / 2) + g * (4 * NB));
+      v[i] = *reinterpret_cast<const uint32_t *>(vp + 4 * b + g * (2 * D) + r * (4 * NB));
+      const u32x2 w = *reinterpret_cast<const u32x2 *>(sp + 8 * NB + 8 * b);
+      s[i][0] = w.x;
+      s[i][1] = w.y;
+    }
+    ks = *reinterpret_cast<const uint32_t *>(sp + 4 * (r < 2 * NB ? r : 2 * NB - 1));
+    // V past the end or of a page that is not there: scale 0 (any bits may lie there)
+    if (there && key + 16 <= len) return;
+    const int32_t at = key + 4 * (int32_t)g;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t keep = there && at + 2 * j < len ? (at + 2 * j + 1 < len ? 0xffffffffu : 0xffffu) : 0;
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) s[i][j] &= keep;
+    }
+  }
+  // Its i-th block as operands, for tile `tile` of a buffer.
+  __device__ inline void put(int i, Buffer<NB, KC> &to, const Masks &m, float fac, uint32_t tile, uint32_t part,
+                             uint32_t lane) const {
+    const uint32_t r = lane & 15, g = lane >> 4, b = block(i, part), y = k[i] >> 8;
+    to.k[tile][b][lane] = (u32x4){as_u32(codes<false>(m, k[i])), as_u32(codes<true>(m, k[i])),
+                                  as_u32(codes<false>(m, y)), as_u32(codes<true>(m, y))};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      u32x2 hi, lo;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t w = v[i] >> (8 * j);
+        const f16x2 n = half ? codes<true>(m, w) : codes<false>(m, w), sc = as_f16x2(s[i][j]), x = n * sc;
+        hi[j] = as_u32(x);
+        lo[j] = as_u32(__builtin_elementwise_fma(n, sc, -x));
+      }
+      reinterpret_cast<u32x2 *>(&to.v[0][tile / 2][2 * b + half][lane])[tile % 2] = hi;
+      reinterpret_cast<u32x2 *>(&to.v[1][tile / 2][2 * b + half][lane])[tile % 2] = lo;
+    }
+    if (i) return;
+    // (the same from each of the tile's waves, and from lanes past the words the last one)
+    const f16x2 w = as_f16x2(ks);
+    const uint32_t n = r < 2 * NB ? r : 2 * NB - 1;
+    *reinterpret_cast<f32x2 *>(&to.ks[tile][n / 2][4 * g + 2 * (n & 1)]) = (f32x2){(float)w.x * fac, (float)w.y * fac};
+    to.there[tile] = there;
+  }
+};
+
+template <int NB, typename T>
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnArgs a) {
+  constexpr int P = sizeof(T) == 4 ? 2 : 1, NW = kPromptWaves;
+  constexpr int D = NB * 32, KC = prompt_keys(D), KT = KC / 16, CT = prompt_tiles(D, sizeof(T) == 4);
+  constexpr uint32_t COLS = NW * CT * 16;
+  typedef Words<NB, KC, NW> Wd;
+  static_assert(NW % KT == 0, "whole waves per tile");
+  __shared__ Buffer<NB, KC> buf[2];
+
+  // the last rows of a sequence first: they see the most keys
+  const uint32_t head = blockIdx.x % a.kv.nkv;
+  const Item t = item_of<COLS>(a, a.items - 1 - blockIdx.x / a.kv.nkv);
+  if (t.none) return;
+  const Kv4Seq &s = t.s;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t r = lane & 15, g = lane >> 4;
+  const uint32_t my_tile = wave / Wd::kPer, part = wave % Wd::kPer;
+  const Masks m = masks();
+  const float fac = __builtin_fmaxf(__builtin_fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
+
+  const int32_t c_end = ((t.first + t.steps) * kKeys + KC - 1) / KC;
+  int32_t c = t.first * kKeys / KC;
+  Wd words;
+  // (past the end the last keys again, into a buffer that nobody reads; the page
+  // number is asked for one step before its words)
+  auto key_of = [&](int32_t n) { return (n < c_end ? n : c_end - 1) * KC + 16 * (int32_t)my_tile; };
+  auto page_of = [&](int32_t n) {
+    const uint32_t i = (uint32_t)key_of(n) >> a.kv.shift;
+    return kv4_const(a.kv.table + (size_t)t.seq * a.kv.max_pages + (i < a.kv.max_pages ? i : 0));
+  };
+  uint32_t page = page_of(c);
+  auto fetch = [&](int32_t n) {
+    words.fetch(a.kv, page, head, key_of(n), s.len, part, lane);
+    page = page_of(n + 1);
+  };
+  auto put = [&](int i, int32_t n) { words.put(i, buf[n & 1], m, fac, my_tile, part, lane); };
+  auto put_all = [&](int32_t n) {
+#pragma unroll
+    for (int i = 0; i < Wd::kBlocks; ++i) put(i, n);
+  };
+  fetch(c);
+
+  // the wave's columns: what each sees, and what all of them see
+  Query<NB, P> Q[CT];
+  Acc<NB> A[CT];
+  int32_t lo[CT], hi[CT], any_lo = s.len, any_hi = 0, all_lo = 0, all_hi = s.len;
+  bool mine[CT];
+  size_t at[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const uint32_t col = t.col0 + (wave * CT + ct) * 16 + r;
+    mine[ct] = col < t.cols;
+    const uint32_t row = mine[ct] ? col / a.group : 0, sub = mine[ct] ? col % a.group : 0;
+    lo[ct] = 0;
+    hi[ct] = s.len;
+    if (a.causal) {
+      const int32_t p = s.pos0 + (int32_t)row;
+      hi[ct] = p + 1 < hi[ct] ? p + 1 : hi[ct];
+      if (a.window && p >= (int32_t)a.window) lo[ct] = p - (int32_t)a.window + 1;
+    }
+    if (!mine[ct]) hi[ct] = 0;
+    at[ct] = (size_t)(s.row0 + row) * a.ldo + (size_t)(head * a.group + sub) * D;
+    const RawQuery<NB, T> raw(static_cast<const T *>(a.q) + (size_t)(s.row0 + row) * a.ldq +
+                              (size_t)(head * a.group + sub) * D + 8 * g);
+    make_query<NB, P, T>(Q[ct], raw, mine[ct], a.scale);
+    Q[ct].fac *= 1 / fac;
+    A[ct].ref = kNever;
+    A[ct].sum = 0;
+#pragma unroll
+    for (int n = 0; n < 2 * NB; ++n) A[ct].o[n] = (f32x4){0, 0, 0, 0};
+  }
+  {
+    const uint32_t first = t.col0 + wave * CT * 16, past = first + CT * 16 < t.cols ? first + CT * 16 : t.cols;
+    if (first < t.cols) {
+      any_lo = 0;
+      any_hi = s.len;
+      if (a.causal) {
+        const int32_t p0 = s.pos0 + (int32_t)(first / a.group), p1 = s.pos0 + (int32_t)((past - 1) / a.group);
+        any_hi = p1 + 1 < any_hi ? p1 + 1 : any_hi;
+        all_hi = p0 + 1 < all_hi ? p0 + 1 : all_hi;
+        if (a.window && p0 >= (int32_t)a.window) any_lo = p0 - (int32_t)a.window + 1;
+        if (a.window && p1 >= (int32_t)a.window) all_lo = p1 - (int32_t)a.window + 1;
+      }
+    }
+  }
+
+  put_all(c);
+  fetch(c + 1);
+  __syncthreads();
+  for (; c < c_end; ++c) {
+    const int32_t key = c * KC;
+    const Buffer<NB, KC> &b_ = buf[c & 1];
+    const bool seen = key < any_hi && key + KC > any_lo;
+    uint32_t p[CT][P][2 * KT];
+    if (seen) {
+    // Scores in stages of up to two blocks of a tile of keys: a stage starts the LDS reads of
+    // the second next one, multiplies, and scales the products of the one before.
+    // (By itself the compiler waits for each read where it is used, and
+    // puts the scales after the branch below, which the empty asm keeps them before.)
+    constexpr int kHalf = (NB + 1) / 2, kStages = 2 * KT;
+    float x[CT][4 * KT];
+    f16x8 kk[3][kHalf];
+    f32x4 sc[3][kHalf], d[2][kHalf][CT];
+    auto read = [&](int st) {
+#pragma unroll
+      for (int h = 0; h < kHalf; ++h) {
+        const int i = st / 2, b = st % 2 * kHalf + h;
+        if (b >= NB) continue;
+        kk[st % 3][h] = __builtin_bit_cast(f16x8, b_.k[i][b][lane]);
+        sc[st % 3][h] = *reinterpret_cast<const f32x4 *>(&b_.ks[i][b][4 * g]);
+      }
+    };
+    auto scaled = [&](int st) {
+#pragma unroll
+      for (int h = 0; h < kHalf; ++h) {
+        const int i = st / 2, b = st % 2 * kHalf + h;
+        if (b >= NB) continue;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float &y = x[ct][4 * i + j];
+            y = b ? __builtin_fmaf(sc[st % 3][h][j], d[st % 2][h][ct][j], y) : sc[st % 3][h][j] * d[st % 2][h][ct][j];
+          }
+      }
+    };
+    read(0);
+    read(1);
+#pragma unroll
+    for (int st = 0; st < kStages; ++st) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < kHalf; ++h) {
+        const int b = st % 2 * kHalf + h;
+        if (b >= NB) continue;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          f32x4 y = {0, 0, 0, 0};
+#pragma unroll
+          for (int p = 0; p < P; ++p) y = mfma(kk[st % 3][h], Q[ct].q[b][p], y);
+          d[st % 2][h][ct] = y;
+        }
+      }
+      if (st) scaled(st - 1);
+      if (st + 2 < kStages) read(st + 2);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    scaled(kStages - 1);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int n = 0; n < 4 * KT; ++n) asm volatile("" : "+v"(x[ct][n]));
+    bool whole = key >= all_lo && key + KC <= all_hi;
+#pragma unroll
+    for (int i = 0; i < KT; ++i) whole = whole && __builtin_amdgcn_readfirstlane(b_.there[i]);
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        const bool there = b_.there[i];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int32_t k = key + 16 * i + 4 * (int32_t)g + j;
+            x[ct][4 * i + j] = k >= lo[ct] && k < hi[ct] && there ? x[ct][4 * i + j] : -__builtin_inff();
+          }
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int n = 0; n < 4 * KT; ++n) {
+        if (P == 2) x[ct][n] *= Q[ct].fac;  // 2^-k of the row
+        top = __builtin_fmaxf(top, x[ct][n]);
+      }
+      if (__any(top > A[ct].ref + kRaise)) {
+        top = max_across(top);
+        const float ref = top > A[ct].ref + kRaise ? top - kLift : A[ct].ref;
+        const float f = __builtin_amdgcn_exp2f(A[ct].ref - ref);
+        A[ct].ref = ref;
+        A[ct].sum *= f;
+        rescale(A[ct], f);
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int n = 0; n < 2 * KT; ++n) {
+        const float x0 = __builtin_amdgcn_exp2f(x[ct][2 * n] - A[ct].ref);
+        const float x1 = __builtin_amdgcn_exp2f(x[ct][2 * n + 1] - A[ct].ref);
+        if (P == 2) {
+          A[ct].sum += x0;
+          A[ct].sum += x1;
+          split_pair(m.minus1, x0, x1, p[ct][0][n], p[ct][P - 1][n]);
+        } else {
+          // the sum of the weights as they are multiplied
+          const f16x2 h = __builtin_convertvector(((f32x2){x0, x1}), f16x2);
+          A[ct].sum = __builtin_amdgcn_fdot2(h, (f16x2){(f16)1.0f, (f16)1.0f}, A[ct].sum, false);
+          p[ct][0][n] = as_u32(h);
+        }
+      }
+    // Products in stages of two tiles of elements, two stages after their reads.
+    constexpr int kV = KT / 2 * NB;  // stages: pairs of key tiles x pairs of element tiles
+    f16x8 v8[3][2][2];
+    auto read_v = [&](int st) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          v8[st % 3][h][e] = __builtin_bit_cast(f16x8, b_.v[h][st / NB][2 * (st % NB) + e][lane]);
+    };
+    read_v(0);
+    read_v(1);
+#pragma unroll
+    for (int st = 0; st < kV; ++st) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 1; h >= 0; --h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            const uint32_t *ph = p[ct][0] + 4 * (st / NB), *pl = p[ct][P - 1] + 4 * (st / NB);
+            f32x4 &o = A[ct].o[2 * (st % NB) + e];
+            o = mfma(v8[st % 3][h][e], as_f16x8(ph[0], ph[1], ph[2], ph[3]), o);
+            if (P == 2 && h == 0) o = mfma(v8[st % 3][0][e], as_f16x8(pl[0], pl[1], pl[2], pl[3]), o);
+          }
+      if (st + 2 < kV) read_v(st + 2);
+      if (st < Wd::kBlocks) put(st, c + 1);
+      if (st == Wd::kBlocks) fetch(c + 2);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    
+    } else {
+      put_all(c + 1);
+      fetch(c + 2);
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const float sum = sum_across(A[ct].sum), inv = sum == 0 ? 0.0f : 1 / sum;
+    if (!mine[ct]) continue;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int e = 0; e < 2 * NB; ++e)
+      *reinterpret_cast<vec4 *>(static_cast<T *>(a.out) + at[ct] + 16 * e + 4 * g) =
+          __builtin_convertvector(A[ct].o[e] * inv, vec4);
+  }
+}
+
 struct Plan {
   uint32_t tiles, groups;  // groups: workgroups that share the steps, 0: one per tile and head
   bool few;                // steps, for which four waves do
+  bool prompt;
   size_t part;             // bytes of a partial result
   size_t starts;           // bytes of the items' starts
   size_t bytes() const { return groups ? groups * 2 * part + starts : 0; }
@@ -797,7 +1146,22 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
   const uint64_t reach = (uint64_t)b->max_pages * c->page;
   uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
   if (window && (uint64_t)window + b->rows + kKeys < len) len = (uint64_t)window + b->rows + kKeys;
-  p.tiles = (uint32_t)(((uint64_t)b->rows * (nh / c->nkv) + kCols - 1) / kCols);
+  const uint64_t cols = (uint64_t)b->rows * (nh / c->nkv);
+  // Prompts where their workgroups fill the device: one of them takes as long for
+  // 64 keys as a wave of the other kernel, of which a CU has 16 (four times as fast
+  // as one), for 5 * 4 of its steps with two tiles of columns per wave, 3 * 4 with one.  (2048 rows over 16384 keys, 8 x 4 heads of 128: 744 us here, 1250 there; four of 224 rows
+  // over as many keys, 20 heads of 64, f32: 17 us here, 10 there.)
+  const uint64_t pcols = (uint64_t)kPromptWaves * 16 * prompt_tiles(c->d, dtype == MADI_F32);
+  const uint64_t ptiles = (cols + pcols - 1) / pcols, steps = (len + kKeys - 1) / kKeys;
+  const uint64_t cost = (len + 63) / 64 * (prompt_tiles(c->d, dtype == MADI_F32) == 2 ? 5 : 3);
+  const uint64_t tiles16 = (cols + kCols - 1) / kCols * c->nkv * b->b;
+  const uint64_t rounds = (ptiles * c->nkv * b->b + cus - 1) / cus;
+  if (rounds * cost < tiles16 * steps / (4 * cus)) {
+    p.prompt = true;
+    p.tiles = (uint32_t)ptiles;
+    return p;
+  }
+  p.tiles = (uint32_t)((cols + kCols - 1) / kCols);
   p.part = (size_t)kCols * (c->d + 2) * 4;
   const uint64_t items = (uint64_t)p.tiles * b->b;
   p.starts = (size_t)(items + 1) * 4;
@@ -811,14 +1175,18 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
 }
 
 template <int NB, typename T>
-void launch(const AttnArgs &a, uint32_t groups, bool few, uint32_t cus) {
+void launch(const AttnArgs &a, const Plan &p, uint32_t cus) {
+  if (p.prompt) {
+    kv4_prompt_kernel<NB, T><<<a.items * a.kv.nkv, 64 * kPromptWaves, 0, stream()>>>(a);
+    return;
+  }
   if (!a.shared) {
     constexpr int W = waves_alone(NB * 32, sizeof(T) == 4);
-    if (few) kv4_attn_kernel<NB, 4, T><<<a.items * a.kv.nkv, 256, 0, stream()>>>(a);
+    if (p.few) kv4_attn_kernel<NB, 4, T><<<a.items * a.kv.nkv, 256, 0, stream()>>>(a);
     else kv4_attn_kernel<NB, W, T><<<a.items * a.kv.nkv, 64 * W, 0, stream()>>>(a);
     return;
   }
-  kv4_attn_kernel<NB, 4, T><<<groups, 256, 0, stream()>>>(a);
+  kv4_attn_kernel<NB, 4, T><<<p.groups, 256, 0, stream()>>>(a);
   const uint64_t cols = (uint64_t)a.kv.rows * a.group;
   const uint32_t tile_cols = cols < kCols ? (uint32_t)cols : kCols;
   const dim3 grid(a.items * tile_cols, a.kv.nkv);
@@ -892,10 +1260,10 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
   const bool f = dtype == MADI_F32;
   const uint32_t cus = (uint32_t)cu_count();
   switch (cache->d) {
-  case 64: f ? launch<2, float>(a, p.groups, p.few, cus) : launch<2, f16>(a, p.groups, p.few, cus); break;
-  case 96: f ? launch<3, float>(a, p.groups, p.few, cus) : launch<3, f16>(a, p.groups, p.few, cus); break;
-  case 128: f ? launch<4, float>(a, p.groups, p.few, cus) : launch<4, f16>(a, p.groups, p.few, cus); break;
-  default: f ? launch<8, float>(a, p.groups, p.few, cus) : launch<8, f16>(a, p.groups, p.few, cus); break;
+  case 64: f ? launch<2, float>(a, p, cus) : launch<2, f16>(a, p, cus); break;
+  case 96: f ? launch<3, float>(a, p, cus) : launch<3, f16>(a, p, cus); break;
+  case 128: f ? launch<4, float>(a, p, cus) : launch<4, f16>(a, p, cus); break;
+  default: f ? launch<8, float>(a, p, cus) : launch<8, f16>(a, p, cus); break;
   }
   return check_launch(what);
 }

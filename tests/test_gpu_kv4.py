@@ -277,6 +277,40 @@ def test_attention(kv4, heads, group, d, page, lens, rows, causal, window, dtype
         check(attend(s, q, nh, dtype, causal, window, reserve=False), want, tol, dtype, "one share:")
 
 
+PROMPTS = [
+    # heads, group, d, page, lens, rows, causal, window: enough columns to fill the device
+    (16, 16, 64, 16, [230, 233], [230, 190], True, 0),
+    (16, 16, 96, 32, [220, 200], [220, 200], True, 0),
+    (16, 16, 128, 64, [250, 230], [230, 230], True, 0),
+    (16, 16, 256, 16, [200, 217], [200, 217], True, 0),
+    (16, 8, 64, 64, [400, 270, 40], [250, 270, 40], True, 70),
+    (8, 32, 64, 16, [70, 129], [250, 129], True, 0),     # rows before the first token
+    (16, 16, 128, 16, [193, 30], [230, 30], False, 0),
+    (20, 1, 64, 64, [1100, 1024], [1100, 1000], True, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,group,d,page,lens,rows,causal,window", PROMPTS)
+def test_prompts(kv4, heads, group, d, page, lens, rows, causal, window, dtype):
+    """Rows enough for the prompts' kernel; a page missing; columns past a
+    tile and rows past the last sequence left alone."""
+    say(f"prompt {heads}x{group}x{d} page {page} lens {lens} rows {rows} causal {causal} window {window} {dtype}")
+    rng = np.random.default_rng(sum(lens) + d + page)
+    s = Setup(kv4, rng, heads, d, page, lens, rows, bad=[(0, 1, 1 << 20)] if page < 64 else ())
+    s.fill(rng)
+    nh = heads * group
+    q = rng.standard_normal((s.m, nh, d), dtype=np.float32).astype(NP[dtype])
+    out = torch.full((s.m + 2, nh * d), 77.0, dtype=getattr(torch, "float16" if dtype == "f16" else "float32"),
+                     device="cuda")
+    want, tol = s.expect(q, nh, causal, window, d ** -0.5, dtype)
+    s.kv4.kvAttn(out, torch.from_numpy(q.reshape(s.m, -1)).cuda(), s.cache, s.batch, nh, causal=causal, window=window)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy()
+    assert (got[s.m:] == 77).all()
+    check(got[:s.m].reshape(s.m, nh, d).astype(np.float64), want, tol, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("qs,ks,scale", [(8.0, 1.0, None), (1.0, 100.0, 0.01), (1e-4, 1.0, 30.0), (300.0, 20.0, 1e-5),
                                          (1.0, 1.0, -0.2), (1.0, 1.0, 0.0)])
