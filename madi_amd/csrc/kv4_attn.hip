@@ -278,10 +278,10 @@ __device__ inline void make_query(Query<NB, P> &Q, const RawQuery<NB, T> &raw, b
   }
 }
 
-// Nibbles 0 and 4 (HIGH: 1 and 5) of w as the codes' values: the f16 numbers
-// 1024 + n (64 + n for the high ones, four bits further up), less 1024 (64) and
-// the codes' 8.  Exact.  The masks are in VGPRs: an instruction reads one SGPR or
-// literal, and v_and_or_b32 wants two constants.
+// Nibbles 0 and 4 (HIGH: 1 and 5) of w as the codes' values in f16, exactly: the
+// numbers 1024 + n (64 + n for the high ones, four bits further up), less
+// 1024 (64) and the codes' 8.  The masks are in VGPRs: an instruction reads one
+// SGPR or literal, and v_and_or_b32 wants two constants.
 struct Masks {
   uint32_t lo, hi;
   float minus1;
@@ -295,6 +295,16 @@ template <bool HIGH>
 __device__ inline f16x2 codes(const Masks &m, uint32_t w) {
   const f16 off = HIGH ? (f16)-72.0f : (f16)-1032.0f;
   return as_f16x2(HIGH ? (w & m.hi) | 0x54005400u : (w & m.lo) | 0x64006400u) + (f16x2){off, off};
+}
+// The same times 2^-9 (kCodeUnit), in two thirds of the time: masked, a nibble is the f16
+// subnormal n 2^-24 (n 2^-20), and one multiply-add makes it (n - 8) 2^-9.  (A
+// v_and_b32 takes half as long as a v_and_or_b32 or a packed f16 instruction.)
+constexpr float kCodeUnit = 0x1p-9f;
+template <bool HIGH>
+__device__ inline f16x2 small_codes(uint32_t w) {
+  const f16 mul = HIGH ? (f16)0x1p11f : (f16)0x1p15f, add = (f16)(-8 * kCodeUnit);
+  return __builtin_elementwise_fma(as_f16x2(w & (HIGH ? 0x00f000f0u : 0x000f000fu)), (f16x2){mul, mul},
+                                   (f16x2){add, add});
 }
 
 // Lane LANE's word, or number, for each of its 16 (row_newbcast).
@@ -316,14 +326,14 @@ __device__ inline void each(F f) {
 
 // Scores of a step, without the factor: x[4i + j] is key 16i + 4g + j.
 template <int NB, int P>
-__device__ inline void scores(float (&x)[8], const Query<NB, P> &Q, const Step<NB> &t, const Masks &m) {
+__device__ inline void scores(float (&x)[8], const Query<NB, P> &Q, const Step<NB> &t) {
   each<NB>([&](auto B) {
     constexpr int b = B();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t w = t.k[i][b], y = w >> 8;
-      const f16x8 kk = as_f16x8(as_u32(codes<false>(m, w)), as_u32(codes<true>(m, w)), as_u32(codes<false>(m, y)),
-                                as_u32(codes<true>(m, y)));
+      const f16x8 kk = as_f16x8(as_u32(small_codes<false>(w)), as_u32(small_codes<true>(w)),
+                                as_u32(small_codes<false>(y)), as_u32(small_codes<true>(y)));
       f32x4 d = {0, 0, 0, 0};
 #pragma unroll
       for (int p = 0; p < P; ++p) d = mfma(kk, Q.q[b][p], d);
@@ -459,7 +469,7 @@ __device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const St
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint32_t w = t.v[i][b] >> (8 * j);
-          v[2 * i + j] = as_u32(half ? codes<true>(m, w) : codes<false>(m, w));
+          v[2 * i + j] = as_u32(half ? small_codes<true>(w) : small_codes<false>(w));
         }
       const f16x8 v8 = as_f16x8(v[0], v[1], v[2], v[3]);
       f32x4 d = A.o[2 * b + half];
@@ -665,6 +675,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
 
       Query<NB, P> Q;
       make_query<NB, P, T>(Q, raw, mine, a.scale);
+      Q.fac /= kCodeUnit;
       Acc<NB> A;
       A.ref = kNever;
       A.sum = 0;
@@ -689,7 +700,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
         const bool whole = key >= all_lo && key + kKeys <= all_hi && st.there[0] && st.there[1];
         if (!whole) cut_scales<NB>(st, key, s.len, r, g);
         float x[8];
-        scores<NB, P>(x, Q, st, m);
+        scores<NB, P>(x, Q, st);
         if (!whole) cut_scores<NB>(x, st, key, lo, hi, g);
         add_values<NB, P>(A, x, Q.fac, st, m);
         at += W;
@@ -702,7 +713,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
       float ref = kNever;
 #pragma unroll
       for (int w = 0; w < W; ++w) ref = __builtin_fmaxf(ref, res.ref[r][w]);
-      const float f = __builtin_amdgcn_exp2f(A.ref - ref), fo = f / A.down;  // (a power of two)
+      const float f = __builtin_amdgcn_exp2f(A.ref - ref), fo = f / (A.down * kCodeUnit);  // (f times a power of two)
       if (g == 0) res.sum[r][wave] = A.sum * f;
       if (mine)
 #pragma unroll
@@ -753,8 +764,14 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(AttnArgs a, uint32_t 
   __shared__ float weight[kMaxGroups], sums[G][D], red[32];
   // the workgroup that began the head has it in its place 1, the others in their place 0
   const float *w = a.work + 2 * (size_t)w0 * kShare<D>;
-  const uint32_t th = threadIdx.x;
+  const uint32_t th = threadIdx.x, grp = th / D, d = th % D;
   auto part = [&](uint32_t n) { return w + (2 * (size_t)n + (n == 0)) * kShare<D>; };
+  // the first O on their way before the weights are known
+  constexpr int kAhead = 8;
+  float ahead[kAhead];
+#pragma unroll
+  for (uint32_t i = 0; i < kAhead; ++i)
+    ahead[i] = grp < G && grp + i * G < count ? part(grp + i * G)[c * D + d] : 0.0f;
   float top = kNever, sum = 0;
   for (uint32_t n = th; n < count; n += TH) top = __builtin_fmaxf(top, weight[n] = part(n)[kCols * D + c]);
   top = wave_max(top);
@@ -770,12 +787,13 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(AttnArgs a, uint32_t 
   sum = wave_sum(sum);
   if (th % 64 == 0) red[16 + th / 64] = sum;
   __syncthreads();
-  const uint32_t grp = th / D, d = th % D;
   if (grp < G) {
     float o = 0;
-#pragma unroll 8
-    for (uint32_t n = grp; n < count; n += G)
-      o = __builtin_fmaf(part(n)[c * D + d], weight[n], o);
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i)
+      if (grp + i * G < count) o = __builtin_fmaf(ahead[i], weight[grp + i * G], o);
+#pragma unroll 4
+    for (uint32_t n = grp + kAhead * G; n < count; n += G) o = __builtin_fmaf(part(n)[c * D + d], weight[n], o);
     sums[grp][d] = o;
   }
   __syncthreads();
