@@ -13,6 +13,18 @@ struct Kv4Args {
   uint32_t n_pages, shift, nkv, max_pages, rows, m;
 };
 
+// A kernel's leading arguments: the hardware preloads the first 16 dwords of scalar
+// arguments into SGPRs, but none of a struct, and a kernel's first loads (a length, a
+// page number) wait for these.  KV4_ARGS passes them, KV4_GATHER puts them back.
+#define KV4_PARAMS                                                                                         \
+  const uint32_t *kv_lens, const uint32_t *kv_row_off, const uint32_t *kv_table, uint8_t *kv_data,         \
+      uint32_t kv_max_pages, uint32_t kv_shift, uint32_t kv_rows, uint32_t kv_m, uint32_t kv_nkv,          \
+      uint32_t kv_n_pages
+#define KV4_ARGS(a) \
+  (a).lens, (a).row_off, (a).table, (a).data, (a).max_pages, (a).shift, (a).rows, (a).m, (a).nkv, (a).n_pages
+#define KV4_GATHER \
+  Kv4Args{kv_data, kv_table, kv_lens, kv_row_off, kv_n_pages, kv_shift, kv_nkv, kv_max_pages, kv_rows, kv_m}
+
 // Checks of the structs, the same for every entry point; fills `a`.
 int kv4_args(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, Kv4Args *a);
 // Checks rows of `width` elements of dtype `ld` apart at p, and tells their

@@ -161,9 +161,10 @@ __device__ inline bool unit_of(const Kv4Args &a, uint32_t per_quad, Unit &u) {
 }
 
 template <int NB, typename T>
-__global__ __launch_bounds__(256) void kv4_store_kernel(Kv4Args a, const T *__restrict__ k,
+__global__ __launch_bounds__(256) void kv4_store_kernel(KV4_PARAMS, const T *__restrict__ k,
                                                         const T *__restrict__ v, uint32_t ldk,
                                                         uint32_t ldv, uint32_t per_quad) {
+  const Kv4Args a = KV4_GATHER;
   Unit u;
   if (!unit_of<NB>(a, per_quad, u) || u.first < 0) return;
   constexpr uint32_t D = NB * 32;
@@ -238,8 +239,9 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(Kv4Args a, const T *__re
 }
 
 template <int NB, typename T>
-__global__ __launch_bounds__(256) void kv4_load_kernel(Kv4Args a, T *__restrict__ k, T *__restrict__ v,
+__global__ __launch_bounds__(256) void kv4_load_kernel(KV4_PARAMS, T *__restrict__ k, T *__restrict__ v,
                                                        uint32_t ldk, uint32_t ldv, uint32_t per_quad) {
+  const Kv4Args a = KV4_GATHER;
   Unit u;
   if (!unit_of<NB>(a, per_quad, u)) return;
   constexpr uint32_t D = NB * 32;
@@ -283,9 +285,9 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4Args a, T *__restrict_
 template <bool STORE, int NB, typename T>
 void launch(const Kv4Args &a, dim3 grid, void *k, void *v, uint32_t ldk, uint32_t ldv, uint32_t per_quad) {
   if constexpr (STORE)
-    kv4_store_kernel<NB, T><<<grid, 256, 0, stream()>>>(a, (const T *)k, (const T *)v, ldk, ldv, per_quad);
+    kv4_store_kernel<NB, T><<<grid, 256, 0, stream()>>>(KV4_ARGS(a), (const T *)k, (const T *)v, ldk, ldv, per_quad);
   else
-    kv4_load_kernel<NB, T><<<grid, 256, 0, stream()>>>(a, (T *)k, (T *)v, ldk, ldv, per_quad);
+    kv4_load_kernel<NB, T><<<grid, 256, 0, stream()>>>(KV4_ARGS(a), (T *)k, (T *)v, ldk, ldv, per_quad);
 }
 
 template <bool STORE>

@@ -67,7 +67,6 @@ struct AttnArgs {
   uint32_t *starts;    // behind them: the items' starts, and the length of a share
   uint32_t ldq, ldo, group, window, causal;
   uint32_t tiles, items;  // column tiles of a sequence; tiles of all sequences
-  uint32_t shared;        // the steps are dealt out evenly (else a workgroup per tile and head)
   float scale;
 };
 
@@ -136,14 +135,13 @@ struct Step {
   bool there[2];
 };
 
-// Page numbers of the tiles at key and key + 16, within the table's reach (the
-// first ones are asked for beside the sequence's length, not after it).
-__device__ inline void find_pages(uint32_t (&page)[2], const Kv4Args &a, uint32_t seq, uint32_t key) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t n = (key + 16 * i) >> a.shift;
-    page[i] = kv4_const(a.table + (size_t)seq * a.max_pages + (n < a.max_pages ? n : 0));
-  }
+// Page numbers of the wave's next kListed steps, two per step, one per lane: `at`
+// is the first step, the others come `stride` apart.  (A scalar load per step
+// would be waited for with the step's LDS reads.)
+constexpr int kListed = 32;
+__device__ inline uint32_t list_pages(const Kv4Args &a, uint32_t seq, uint32_t at, uint32_t stride, uint32_t lane) {
+  const uint32_t n = ((at + (lane >> 1) * stride) * kKeys + (lane & 1) * 16) >> a.shift;
+  return kv4_const(a.table + (size_t)seq * a.max_pages + (n < a.max_pages ? n : 0));
 }
 
 // A wave's ring of steps in LDS.  Every lane reads back what it loaded itself,
@@ -159,11 +157,12 @@ struct Ring {
 };
 template <int NB>
 __device__ inline void load_pieces(const uint8_t *from, uint32_t voff, uint32_t to) {
-#pragma unroll
-  for (int n = 0; n < Ring<NB>::kWide; ++n) global_dma<16>(from + 16 * n, voff, to + 1024 * n);
-#pragma unroll
-  for (int n = 0; n < Ring<NB>::kNarrow; ++n)
-    global_dma<4>(from + 16 * Ring<NB>::kWide + 4 * n, voff, to + 1024 * Ring<NB>::kWide + 256 * n);
+  constexpr int W = Ring<NB>::kWide, N = Ring<NB>::kNarrow;
+  if constexpr (W > 0) global_dma<16>(from, voff, to);
+  if constexpr (W > 1) global_dma<16, 16>(from, voff, to + 1024 - 16);
+  if constexpr (N > 0) global_dma<4, 16 * W>(from, voff, to + 1024 * W - 16 * W);
+  if constexpr (N > 1) global_dma<4, 16 * W + 4>(from, voff, to + 1024 * W + 256 - (16 * W + 4));
+  if constexpr (N > 2) global_dma<4, 16 * W + 8>(from, voff, to + 1024 * W + 512 - (16 * W + 8));
 }
 template <int NB>
 __device__ inline void read_pieces(uint32_t (&w)[NB], const uint8_t *from, uint32_t lane) {
@@ -185,6 +184,7 @@ __device__ inline uint32_t fetch(const Kv4Args &a, const uint32_t (&pages)[2], u
                                  uint32_t lane, uint32_t to) {
   constexpr uint32_t D = NB * 32;
   const uint32_t r = lane & 15, g = lane >> 4;
+  const uint32_t kv = r * (D / 2) + g * (4 * NB), vv = ((D / 2) << a.shift) + g * (2 * D) + r * (4 * NB);
   uint32_t there = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -193,15 +193,14 @@ __device__ inline uint32_t fetch(const Kv4Args &a, const uint32_t (&pages)[2], u
     there |= ok ? 1u << i : 0;
     const uint32_t off = (uint32_t)(key + 16 * i) & ((1u << a.shift) - 1);
     const uint8_t *blk = kv4_block(a, ok ? pages[i] : 0, head, D);
-    const uint8_t *v = blk + ((size_t)(D / 2) << a.shift) + (size_t)off * (D / 2);
-    const uint8_t *sc = blk + ((size_t)D << a.shift) + (size_t)off * (D / 8);
     const uint32_t at = to + i * Ring<NB>::kTile;
-    load_pieces<NB>(blk + (size_t)off * (D / 2), r * (D / 2) + g * (4 * NB), at);
-    load_pieces<NB>(v, g * (2 * D) + r * (4 * NB), at + 256 * NB);
+    load_pieces<NB>(blk, kv + off * (D / 2), at);
+    load_pieces<NB>(blk, vv + off * (D / 2), at + 256 * NB);
 #pragma unroll
     for (uint32_t n = 0; n < Ring<NB>::kScales; ++n) {
       const uint32_t w = 16 * n + r;  // (nb < 4: lanes past the words hold the last one)
-      global_dma<4>(sc, g * (D / 2) + 4 * (w < 4 * NB ? w : 4 * NB - 1), at + 512 * NB + 256 * n);
+      global_dma<4>(blk, (D << a.shift) + g * (D / 2) + 4 * (w < 4 * NB ? w : 4 * NB - 1) + off * (D / 8),
+                    at + 512 * NB + 256 * n);
     }
   }
   return there;
@@ -540,15 +539,16 @@ __device__ inline uint32_t wave_scan(uint32_t v) {
 // W waves on the same 16 columns, wave w taking steps w, w + W, .. of the
 // workgroup's segments.
 //
-// shared: the steps of all items and heads in a row (item by item, head by
+// SHARED: the steps of all items and heads in a row (item by item, head by
 // head, each after kOverhead empty places) are dealt out to the workgroups in
 // equal shares, however long the sequences are; a share may hold several
 // segments, and a segment that is not a whole item and head goes into the workspace
 // for kv4_attn_join_kernel.  A workgroup has two places there: 0 for
 // a segment that others began, 1 for one that it begins and does not end.
 // Else: a workgroup per item and head.
-template <int NB, int W, typename T>
-__global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4_attn_kernel(AttnArgs a) {
+template <int NB, int W, bool SHARED, typename T>
+__global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4_attn_kernel(KV4_PARAMS, AttnArgs a) {
+  a.kv = KV4_GATHER;
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
   constexpr int D = NB * 32;
   constexpr int R = NB == 2 && W == 4 ? 4 : 2;  // as deep as LDS lets the waves be
@@ -568,7 +568,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
 
   // The workgroup's part [at, end) of the row, from place `in` of item `item`
   uint32_t item, in, left;
-  if (a.shared) {
+  if (SHARED) {
     // The length of all items, then the one that holds place `from`; every wave
     // by itself, 64 items at a time (up to 64, both from one scan).
     uint32_t total = 0, upto = 0, len = 0;
@@ -607,12 +607,16 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
     in = blockIdx.x % a.kv.nkv;  // of heads
     left = 1;
   }
+  // (without a window the steps begin at 0: the pages are asked for beside the
+  // length, not after it)
+  uint32_t listed = 0;
+  if (!SHARED && !a.window) listed = list_pages(a.kv, a.tiles == 1 ? item : item / a.tiles, wave, W, lane);
 
   for (; item < a.items && left; ++item, in = 0) {
     const Item t = item_of(a, item);
     const Kv4Seq &s = t.s;
     if (t.none) {
-      if (a.shared) continue;
+      if (SHARED) continue;
       return;
     }
     // keys every column of the tile sees
@@ -636,12 +640,12 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
     if (!mine) hi = 0;
 
     const uint32_t length = (uint32_t)t.steps + kOverhead;
-    uint32_t head = a.shared ? in / length : in, place = a.shared ? in - head * length : 0;
+    uint32_t head = SHARED ? in / length : in, place = SHARED ? in - head * length : 0;
     for (; head < a.kv.nkv && left; ++head, place = 0) {
       // the segment: steps [begin, end) of the head's t.steps
       int32_t begin = 0, end = t.steps;
       bool last = true;  // of the head
-      if (a.shared) {
+      if (SHARED) {
         const uint32_t n = length - place < left ? length - place : left;
         last = place + n == length;
         begin = place > kOverhead ? (int32_t)(place - kOverhead) : 0;
@@ -655,16 +659,22 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
 
       int32_t at = begin + (int32_t)wave, issued = at;
       uint32_t slot_in = 0, there_in = 0;  // next slot to load; which tiles of the ring's slots have pages
-      uint32_t pages[2];
-      find_pages(pages, a.kv, t.seq, (t.first + issued) * kKeys);
+      int32_t next = 0;  // in the list of pages
+      if (SHARED || a.window) listed = list_pages(a.kv, t.seq, (uint32_t)(t.first + at), W, lane);
       auto issue = [&]() {
         if (issued < end) {
+          if (next == kListed) {
+            listed = list_pages(a.kv, t.seq, (uint32_t)(t.first + issued), W, lane);
+            next = 0;
+          }
+          const uint32_t pages[2] = {(uint32_t)__builtin_amdgcn_readlane(listed, 2 * next),
+                                     (uint32_t)__builtin_amdgcn_readlane(listed, 2 * next + 1)};
+          ++next;
           const uint32_t ok = fetch<NB>(a.kv, pages, head, (t.first + issued) * kKeys, s.len, lane,
                                         ring_at + slot_in * Ring<NB>::kBytes);
           there_in = (there_in & ~(3u << (2 * slot_in))) | ok << (2 * slot_in);
           slot_in = slot_in + 1 == R ? 0 : slot_in + 1;
           issued += W;
-          find_pages(pages, a.kv, t.seq, (t.first + issued) * kKeys);
         }
       };
       // (the queries are asked for first: theirs is the shorter way)
@@ -752,7 +762,8 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
 // than one: a workgroup per item and column, and head.  The segments' weights
 // first, then D threads add up their O, TH / D groups of them every so many segments.
 template <int NB, int TH, typename T>
-__global__ __launch_bounds__(TH) void kv4_attn_join_kernel(AttnArgs a, uint32_t tile_cols) {
+__global__ __launch_bounds__(TH) void kv4_attn_join_kernel(KV4_PARAMS, AttnArgs a, uint32_t tile_cols) {
+  a.kv = KV4_GATHER;
   constexpr int D = NB * 32, G = TH / D;
   const uint32_t item = blockIdx.x / tile_cols, c = blockIdx.x % tile_cols, head = blockIdx.y;
   const Item t = item_of(a, item);
@@ -898,7 +909,8 @@ struct Words {
 };
 
 template <int NB, typename T>
-__global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PARAMS, AttnArgs a) {
+  a.kv = KV4_GATHER;
   constexpr int P = sizeof(T) == 4 ? 2 : 1, NW = kPromptWaves;
   constexpr int D = NB * 32, KC = prompt_keys(D), KT = KC / 16, CT = prompt_tiles(D, sizeof(T) == 4);
   constexpr uint32_t COLS = NW * CT * 16;
@@ -1152,7 +1164,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 
 struct Plan {
   uint32_t tiles, groups;  // groups: workgroups that share the steps, 0: one per tile and head
-  bool few;                // steps, for which four waves do
+  bool few;                // steps (up to eight)
   bool prompt;
   size_t part;             // bytes of a partial result
   size_t starts;           // bytes of the items' starts
@@ -1195,24 +1207,28 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
 template <int NB, typename T>
 void launch(const AttnArgs &a, const Plan &p, uint32_t cus) {
   if (p.prompt) {
-    kv4_prompt_kernel<NB, T><<<a.items * a.kv.nkv, 64 * kPromptWaves, 0, stream()>>>(a);
+    kv4_prompt_kernel<NB, T><<<a.items * a.kv.nkv, 64 * kPromptWaves, 0, stream()>>>(KV4_ARGS(a.kv), a);
     return;
   }
-  if (!a.shared) {
+  if (!p.groups) {
     constexpr int W = waves_alone(NB * 32, sizeof(T) == 4);
-    if (p.few) kv4_attn_kernel<NB, 4, T><<<a.items * a.kv.nkv, 256, 0, stream()>>>(a);
-    else kv4_attn_kernel<NB, W, T><<<a.items * a.kv.nkv, 64 * W, 0, stream()>>>(a);
+    // few steps: a wave each while a workgroup has a CU for itself, else four waves
+    if (p.few && a.items * a.kv.nkv <= 2 * cus)
+      kv4_attn_kernel<NB, 8, false, T><<<a.items * a.kv.nkv, 512, 0, stream()>>>(KV4_ARGS(a.kv), a);
+    else if (p.few)
+      kv4_attn_kernel<NB, 4, false, T><<<a.items * a.kv.nkv, 256, 0, stream()>>>(KV4_ARGS(a.kv), a);
+    else kv4_attn_kernel<NB, W, false, T><<<a.items * a.kv.nkv, 64 * W, 0, stream()>>>(KV4_ARGS(a.kv), a);
     return;
   }
-  kv4_attn_kernel<NB, 4, T><<<p.groups, 256, 0, stream()>>>(a);
+  kv4_attn_kernel<NB, 4, true, T><<<p.groups, 256, 0, stream()>>>(KV4_ARGS(a.kv), a);
   const uint64_t cols = (uint64_t)a.kv.rows * a.group;
   const uint32_t tile_cols = cols < kCols ? (uint32_t)cols : kCols;
   const dim3 grid(a.items * tile_cols, a.kv.nkv);
   // few columns are of long caches, many segments each; of many most have one
   if ((uint64_t)grid.x * grid.y <= 2 * cus)
-    kv4_attn_join_kernel<NB, 1024, T><<<grid, 1024, 0, stream()>>>(a, tile_cols);
+    kv4_attn_join_kernel<NB, 1024, T><<<grid, 1024, 0, stream()>>>(KV4_ARGS(a.kv), a, tile_cols);
   else
-    kv4_attn_join_kernel<NB, 256, T><<<grid, 256, 0, stream()>>>(a, tile_cols);
+    kv4_attn_join_kernel<NB, 256, T><<<grid, 256, 0, stream()>>>(KV4_ARGS(a.kv), a, tile_cols);
 }
 
 }  // namespace
@@ -1272,7 +1288,6 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
   a.causal = (uint32_t)causal;
   a.tiles = p.tiles;
   a.items = (uint32_t)items;
-  a.shared = p.groups != 0;
   a.starts = reinterpret_cast<uint32_t *>(a.work + p.groups * 2 * (p.part / 4));
   a.scale = scale;
   const bool f = dtype == MADI_F32;

@@ -58,20 +58,21 @@ __device__ inline void dma16(desc_t d, uint32_t voff, uint32_t soff, uint32_t m0
     asm volatile("buffer_load_dwordx4 %0, %1, %2 offen offset:%3 lds"
                  ::"v"(voff), "s"(d), "s"(sgpr(soff)), "n"(OFF), "{m0}"(sgpr(m0)) : "memory");
 }
-// The same from a global address: SIZE (4 or 16) bytes per lane at base + voff
-// -> LDS m0 + SIZE * lane, base uniform.  The LDS reads before it are waited
-// for, so that it may overwrite what they read.
-template <int SIZE>
+// The same from a global address: SIZE (4 or 16) bytes per lane at base + voff + OFF
+// -> LDS m0 + OFF + SIZE * lane, base uniform.  The LDS reads before it are
+// waited for, so that it may overwrite what they read.
+template <int SIZE, int OFF = 0>
 __device__ inline void global_dma(const void *base, uint32_t voff, uint32_t m0) {
   static_assert(SIZE == 4 || SIZE == 16, "bytes per lane");
+  static_assert(OFF >= 0 && OFF < 4096, "instruction offset range");
   const uint64_t b = reinterpret_cast<uint64_t>(base);
   const uint64_t sb = (uint64_t)sgpr((uint32_t)(b >> 32)) << 32 | sgpr((uint32_t)b);
   if constexpr (SIZE == 16)
-    asm volatile("s_nop 0\n\ts_waitcnt lgkmcnt(0)\n\tglobal_load_lds_dwordx4 %0, %1"
-                 ::"v"(voff), "s"(sb), "{m0}"(sgpr(m0)) : "memory");
+    asm volatile("s_nop 0\n\ts_waitcnt lgkmcnt(0)\n\tglobal_load_lds_dwordx4 %0, %1 offset:%2"
+                 ::"v"(voff), "s"(sb), "n"(OFF), "{m0}"(sgpr(m0)) : "memory");
   else
-    asm volatile("s_nop 0\n\ts_waitcnt lgkmcnt(0)\n\tglobal_load_lds_dword %0, %1"
-                 ::"v"(voff), "s"(sb), "{m0}"(sgpr(m0)) : "memory");
+    asm volatile("s_nop 0\n\ts_waitcnt lgkmcnt(0)\n\tglobal_load_lds_dword %0, %1 offset:%2"
+                 ::"v"(voff), "s"(sb), "n"(OFF), "{m0}"(sgpr(m0)) : "memory");
 }
 // Until at most N of this wave's vector-memory ops are outstanding.
 template <int N>

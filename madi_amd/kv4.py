@@ -56,6 +56,7 @@ class KV4:
         if not data.is_contiguous() or _bytes(n_pages, page, heads, dim) > held:
             raise MadiError(-5, "kv4.KV4", f"data must be contiguous and hold {n_pages} pages, has {held} bytes")
         self.data, self.page, self.heads, self.dim, self.n_pages = data, page, heads, dim, n_pages
+        self.width, self.scale = heads * dim, 1.0 / math.sqrt(dim)
         self._c = _Cache(data.data_ptr(), n_pages, page, heads, dim)
         self.addr = ctypes.addressof(self._c)
 
@@ -113,45 +114,41 @@ class Batch:
         return need
 
 
-_DTYPES: dict = {}
+_check: tuple = ()
 
 
-def _rows(t, m: int, width: int, what: str):
-    """(row distance, dtype code) of rows [m][width]."""
-    if not _DTYPES:
+def _rows(t, m: int, width: int, what: str) -> int:
+    """2 * row distance + dtype code of rows [m][width].  (Rows that are not apart, a
+    broadcast's, are left to the library to refuse.)"""
+    global _check
+    if not _check:
         import torch
-        _DTYPES.update({torch.float16: F16, torch.float32: F32})
-    code = _DTYPES.get(t.dtype)
-    shape, st = t.shape, t.stride()
-    n = len(shape)
-    if n == 2:
-        ok = shape[1] == width and st[1] == 1
-    else:
-        ok = n == 3 and shape[1] * shape[2] == width and st[2] == 1 and (st[1] == shape[2] or shape[1] == 1)
-    if code is None or not ok or shape[0] < m:
+        from ._pycall import rows
+        _check = rows, torch.float16, torch.float32
+    rows, f16, f32 = _check
+    r = rows(t, m, width, f16, f32)
+    if r < 0:
         raise MadiError(-5, what, f"rows must be float16 or float32 [{m}][{width}] with contiguous rows; "
-                                  f"got {t.dtype} {tuple(shape)} with strides {st}")
-    # rows that are not apart (a broadcast) are left to the library to refuse; one row has no distance
-    return (st[0] if shape[0] > 1 else max(st[0], width)), code
+                                  f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    return r
+
+
+def _pair(a, b, m: int, width: int, what: str):
+    a, b = _rows(a, m, width, what), _rows(b, m, width, what)
+    if (a ^ b) & 1:
+        raise MadiError(-9, what, "the two tensors are of two types")
+    return a >> 1, b >> 1, a & 1
 
 
 def kvStore(cache: KV4, batch: Batch, k, v) -> None:
     """Quantise rows k, v into the cache, at each sequence's last positions."""
-    w = cache.heads * cache.dim
-    ldk, dt = _rows(k, batch.m, w, "kvStore")
-    ldv, dv = _rows(v, batch.m, w, "kvStore")
-    if dt != dv:
-        raise MadiError(-9, "kvStore", "k and v are of two types")
+    ldk, ldv, dt = _pair(k, v, batch.m, cache.width, "kvStore")
     calls.madi_kv4_store(cache.addr, batch.addr, k, v, ldk, ldv, dt)
 
 
 def kvLoad(cache: KV4, batch: Batch, k, v) -> None:
     """Read each sequence's last rows back into k, v."""
-    w = cache.heads * cache.dim
-    ldk, dt = _rows(k, batch.m, w, "kvLoad")
-    ldv, dv = _rows(v, batch.m, w, "kvLoad")
-    if dt != dv:
-        raise MadiError(-9, "kvLoad", "k and v are of two types")
+    ldk, ldv, dt = _pair(k, v, batch.m, cache.width, "kvLoad")
     calls.madi_kv4_load(k, v, ldk, ldv, dt, cache.addr, batch.addr)
 
 
@@ -160,13 +157,9 @@ def kvAttn(out, q, cache: KV4, batch: Batch, nh: int, causal: bool = True, windo
     """out = softmax(scale q K^T) V over the cache, scale 1 / sqrt(dim) by
     default.  causal: a row sees the positions up to its own, the last `window`
     of them where window is not 0; else all of its sequence (cross-attention)."""
-    w = nh * cache.dim
-    ldq, dt = _rows(q, batch.m, w, "kvAttn")
-    ldo, do = _rows(out, batch.m, w, "kvAttn")
-    if dt != do:
-        raise MadiError(-9, "kvAttn", "q and out are of two types")
+    ldo, ldq, dt = _pair(out, q, batch.m, nh * cache.dim, "kvAttn")
     calls.madi_kv4_attn(out, q, cache.addr, batch.addr, nh, ldo, ldq, window, 1 if causal else 0, dt,
-                        1.0 / math.sqrt(cache.dim) if scale is None else scale)
+                        cache.scale if scale is None else scale)
 
 
 __all__ = ["KV4", "Batch", "alloc", "kvStore", "kvLoad", "kvAttn", "F16", "F32"]
