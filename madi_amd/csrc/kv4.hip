@@ -2,11 +2,12 @@
 // madi_kv4_load; the format and the layout are in madi_q8.h).
 //
 // A unit of work is four consecutive tokens (4u..4u+3 of a sequence) of one
-// block of one head of K or V: 128 elements, 16 lanes of 8, so that a V word
-// (four tokens' bytes) is made in one place.  Lane l of the 16 has token l & 3
-// and elements 32b + 8g .. + 7, g = 2 (l >> 2 & 1) + (l >> 3): with this order
-// the V words come out of two byte transposes between neighbouring lanes
-// (DPP) instead of through LDS.
+// block of one head, first of K, then of V: 2 x 128 elements, 16 lanes of 8, so
+// that a V word (four tokens' bytes) is made in one place.  Lane l of the 16 has
+// token l & 3 and elements 32b + 8g .. + 7, g = 2 (l >> 2 & 1) + (l >> 3): with
+// this order the V words come out of two byte transposes between neighbouring lanes
+// (DPP) instead of through LDS.  Both are bound by memory: K's and V's loads are
+// in flight together.
 #include "kv4.h"
 
 using namespace madi;
@@ -106,15 +107,17 @@ __device__ inline void load8(const f16 *p, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
 }
+// (not kept in the L2, which the rows mostly exceed: 131072 rows of 8 heads of 128 read
+// back in 173 us, 184 with ordinary stores)
 __device__ inline void store8(float *p, const float (&x)[8]) {
-  *reinterpret_cast<f32x4 *>(p) = (f32x4){x[0], x[1], x[2], x[3]};
-  *reinterpret_cast<f32x4 *>(p + 4) = (f32x4){x[4], x[5], x[6], x[7]};
+  __builtin_nontemporal_store((f32x4){x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4 *>(p));
+  __builtin_nontemporal_store((f32x4){x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4 *>(p + 4));
 }
 __device__ inline void store8(f16 *p, const float (&x)[8]) {
   f16x8 v;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = (f16)x[i];
-  *reinterpret_cast<f16x8 *>(p) = v;
+  __builtin_nontemporal_store(v, reinterpret_cast<f16x8 *>(p));
 }
 
 // The code of x (plus 8) against scale s > 0: |x| / s to the nearest whole
@@ -133,51 +136,34 @@ __device__ inline uint32_t code(float x, float s, float inv, float half) {
 
 struct Unit {
   uint32_t seq, h, b, g, tok, col;  // col: first of the lane's 8 elements in a row
-  bool v;
-  int32_t pos;   // of the lane's token
-  int32_t first; // of token 0
+  int32_t pos;    // of the lane's token
+  int32_t first;  // of token 0
+  bool mine;      // the lane's token is one of the call's rows
+  size_t row;     // and that row
   Kv4Seq s;
 };
 // The calling lane's unit; false where the workgroup or the lane has none.
 template <int NB>
 __device__ inline bool unit_of(const Kv4Args &a, uint32_t per_quad, Unit &u) {
   const uint32_t quad = blockIdx.x / per_quad, part = blockIdx.x % per_quad;
-  const uint32_t l = threadIdx.x & 15, n = part * 16 + (threadIdx.x >> 4);
+  const uint32_t l = threadIdx.x & 15, hb = part * 16 + (threadIdx.x >> 4);
   u.seq = blockIdx.y;
   u.s = kv4_seq(a, u.seq);
   u.first = ((u.s.pos0 >> 2) + (int32_t)quad) * 4;
-  if (u.first >= u.s.pos0 + (int32_t)u.s.nrows) return false;
-  const uint32_t blocks = a.nkv * NB;
-  if (n >= 2 * blocks) return false;
-  u.v = n >= blocks;
-  const uint32_t hb = u.v ? n - blocks : n;
+  if (u.first >= u.s.pos0 + (int32_t)u.s.nrows || hb >= a.nkv * NB) return false;
   u.h = hb / NB;
   u.b = hb % NB;
   u.tok = l & 3;
   u.g = (l >> 2 & 1) * 2 + (l >> 3);
   u.col = hb * 32 + u.g * 8;
   u.pos = u.first + (int32_t)u.tok;
+  u.mine = u.pos >= u.s.pos0 && u.pos < u.s.pos0 + (int32_t)u.s.nrows;
+  u.row = u.s.row0 + (uint32_t)(u.pos - u.s.pos0);
   return true;
 }
 
-template <int NB, typename T>
-__global__ __launch_bounds__(256) void kv4_store_kernel(KV4_PARAMS, const T *__restrict__ k,
-                                                        const T *__restrict__ v, uint32_t ldk,
-                                                        uint32_t ldv, uint32_t per_quad) {
-  const Kv4Args a = KV4_GATHER;
-  Unit u;
-  if (!unit_of<NB>(a, per_quad, u) || u.first < 0) return;
-  constexpr uint32_t D = NB * 32;
-  const uint32_t l = threadIdx.x & 15;
-  // a unit of four tokens lies in one page
-  const uint32_t page = kv4_page(a, u.seq, u.first);
-  if (page >= a.n_pages) return;
-  const bool mine = u.pos >= u.s.pos0 && u.pos < u.s.pos0 + (int32_t)u.s.nrows;
-  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (mine) {
-    const size_t row = u.s.row0 + (uint32_t)(u.pos - u.s.pos0);
-    load8(u.v ? v + row * ldv + u.col : k + row * ldk + u.col, x);
-  }
+// The codes (plus 8, a byte each) of the lane's 8 elements and their block's scale.
+__device__ inline f16 quantise(float (&x)[8], uint32_t &lo, uint32_t &hi) {
   float top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -190,7 +176,7 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(KV4_PARAMS, const T *__r
   f16 sh = (f16)(top / 7.0f);
   if (!(sh <= (f16)9352.0f)) sh = (f16)9352.0f;
   const float s = (float)sh;
-  uint32_t lo = 0x08080808u, hi = 0x08080808u;  // codes of elements 0-3 and 4-7, a byte each
+  lo = hi = 0x08080808u;
   if (s > 0) {
     const float inv = __builtin_amdgcn_rcpf(s), half = 0.5f * s;
     lo = hi = 0;
@@ -200,42 +186,75 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(KV4_PARAMS, const T *__r
       hi |= code(x[4 + i], s, inv, half) << (8 * i);
     }
   }
+  return sh;
+}
 
+template <int NB, typename T>
+__global__ __launch_bounds__(256) void kv4_store_kernel(KV4_PARAMS, const T *__restrict__ k,
+                                                        const T *__restrict__ v, uint32_t ldk,
+                                                        uint32_t ldv, uint32_t per_quad) {
+  const Kv4Args a = KV4_GATHER;
+  Unit u;
+  if (!unit_of<NB>(a, per_quad, u) || u.first < 0) return;
+  constexpr uint32_t D = NB * 32;
+  const uint32_t l = threadIdx.x & 15;
+  // a unit of four tokens lies in one page; its number and the rows are asked for together
+  const uint32_t page = kv4_page(a, u.seq, u.first);
+  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (u.mine) {
+    load8(k + u.row * ldk + u.col, x);
+    load8(v + u.row * ldv + u.col, y);
+  }
+  if (page >= a.n_pages) return;
   uint8_t *blk = kv4_block(a, page, u.h, D);
   const uint32_t off = (uint32_t)u.pos & ((1u << a.shift) - 1), four = off >> 2;
-  if (mine && u.g == 0) {
-    uint8_t *sc = blk + ((size_t)D << a.shift) + (size_t)four * (D / 2);
-    reinterpret_cast<f16 *>(sc)[((u.v ? NB : 0) + u.b) * 4 + u.tok] = sh;
+  f16 *sc = reinterpret_cast<f16 *>(blk + ((size_t)D << a.shift) + (size_t)four * (D / 2)) + u.b * 4 + u.tok;
+
+  uint32_t lo, hi;
+  f16 s = quantise(x, lo, hi);
+  // K: element 2j in nibble j, element 2j+1 in nibble 4+j
+  const uint32_t ev = __builtin_amdgcn_perm(hi, lo, 0x06040200u);  // bytes e0 e2 e4 e6
+  const uint32_t od = __builtin_amdgcn_perm(hi, lo, 0x07050301u);  // bytes e1 e3 e5 e7
+  const uint32_t evn = ev | ev >> 4, odn = od | od >> 4;           // nibble pairs in bytes 0, 2
+  if (u.mine) {
+    if (u.g == 0) sc[0] = s;
+    *reinterpret_cast<uint32_t *>(blk + (size_t)off * (D / 2) + (u.g * NB + u.b) * 4) =
+        __builtin_amdgcn_perm(odn, evn, 0x06040200u);
   }
-  if (!u.v) {
-    // element 2j in nibble j, element 2j+1 in nibble 4+j
-    const uint32_t ev = __builtin_amdgcn_perm(hi, lo, 0x06040200u);  // bytes e0 e2 e4 e6
-    const uint32_t od = __builtin_amdgcn_perm(hi, lo, 0x07050301u);  // bytes e1 e3 e5 e7
-    const uint32_t evn = ev | ev >> 4, odn = od | od >> 4;           // nibble pairs in bytes 0, 2
-    const uint32_t w = __builtin_amdgcn_perm(odn, evn, 0x06040200u);
-    if (mine)
-      *reinterpret_cast<uint32_t *>(blk + (size_t)off * (D / 2) + (u.g * NB + u.b) * 4) = w;
+
+  s = quantise(y, lo, hi);
+  if (u.mine && u.g == 0) sc[4 * NB] = s;
+  // V: lanes 8i + 0..3 have the low nibbles of 8 words, lanes 8i + 4..7 the high
+  // ones of the same 8: they exchange four words' worth, then four lanes (the
+  // four tokens) transpose, and lane l has word (c = l, b).
+  const uint32_t odd = l & 4;
+  const uint32_t got = lane_xor4(odd ? lo : hi);
+  uint32_t w = odd ? (got | hi << 4) : (lo | got << 4);
+  w = token_order(transpose4(w, l));
+  uint8_t *dst = blk + ((size_t)(D / 2) << a.shift) + (size_t)four * (2 * D) + (l * NB + u.b) * 4;
+  // tokens of this store among the four
+  const int32_t lo_t = u.s.pos0 - u.first, hi_t = lo_t + (int32_t)u.s.nrows;
+  if (lo_t <= 0 && hi_t >= 4) {
+    *reinterpret_cast<uint32_t *>(dst) = w;
   } else {
-    // Lanes 8i + 0..3 have the low nibbles of 8 words, lanes 8i + 4..7 the high
-    // ones of the same 8: they exchange four words' worth, then four lanes (the
-    // four tokens) transpose, and lane l has word (c = l, b).
-    const uint32_t odd = l & 4;
-    const uint32_t got = lane_xor4(odd ? lo : hi);
-    uint32_t w = odd ? (got | hi << 4) : (lo | got << 4);
-    w = token_order(transpose4(w, l));
-    uint8_t *dst = blk + ((size_t)(D / 2) << a.shift) + (size_t)four * (2 * D) + (l * NB + u.b) * 4;
-    // tokens of this store among the four
-    const int32_t lo_t = u.s.pos0 - u.first, hi_t = lo_t + (int32_t)u.s.nrows;
-    if (lo_t <= 0 && hi_t >= 4) {
-      *reinterpret_cast<uint32_t *>(dst) = w;
-    } else {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int byte = (t & 1) * 2 + (t >> 1);
-        if (t >= lo_t && t < hi_t) dst[byte] = (uint8_t)(w >> (8 * byte));
-      }
+    for (int t = 0; t < 4; ++t) {
+      const int byte = (t & 1) * 2 + (t >> 1);
+      if (t >= lo_t && t < hi_t) dst[byte] = (uint8_t)(w >> (8 * byte));
     }
   }
+}
+
+// Codes (plus 8, a byte each) times the scale.
+template <typename T>
+__device__ inline void put_row(T *p, uint32_t lo, uint32_t hi, float s) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = (float)((int)(lo >> (8 * i) & 0xffu) - 8) * s;
+    x[4 + i] = (float)((int)(hi >> (8 * i) & 0xffu) - 8) * s;
+  }
+  store8(p, x);
 }
 
 template <int NB, typename T>
@@ -248,38 +267,26 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(KV4_PARAMS, T *__restrict
   const uint32_t l = threadIdx.x & 15;
   uint32_t page = 0xffffffffu;
   if (u.first >= 0) page = kv4_page(a, u.seq, u.first);  // below 0 there is none
-  uint32_t lo = 0x08080808u, hi = 0x08080808u;
-  float s = 0;
-  if (page < a.n_pages) {  // the same for the 16 lanes
+  uint32_t kw = 0x88888888u, vw = 0x88888888u;
+  float ks = 0, vs = 0;
+  if (page < a.n_pages) {
     const uint8_t *blk = kv4_block(a, page, u.h, D);
-    const uint32_t off0 = (uint32_t)u.first & ((1u << a.shift) - 1), four = off0 >> 2;
-    const uint8_t *sc = blk + ((size_t)D << a.shift) + (size_t)four * (D / 2);
-    s = (float)reinterpret_cast<const f16 *>(sc)[((u.v ? NB : 0) + u.b) * 4 + u.tok];
-    if (!u.v) {
-      const uint32_t w = *reinterpret_cast<const uint32_t *>(blk + (size_t)(off0 + u.tok) * (D / 2) +
-                                                             (u.g * NB + u.b) * 4);
-      const uint32_t a0 = w & 0x0f0f0f0fu, a1 = (w >> 4) & 0x0f0f0f0fu;  // e0 e4 e1 e5, e2 e6 e3 e7
-      lo = __builtin_amdgcn_perm(a1, a0, 0x06040200u);
-      hi = __builtin_amdgcn_perm(a1, a0, 0x07050301u);
-    } else {
-      uint32_t w = *reinterpret_cast<const uint32_t *>(blk + ((size_t)(D / 2) << a.shift) +
-                                                       (size_t)four * (2 * D) + (l * NB + u.b) * 4);
-      w = transpose4(token_order(w), l);  // the lane's token of words c = 4 (l >> 2) + 0..3
-      const uint32_t low = w & 0x0f0f0f0fu, high = (w >> 4) & 0x0f0f0f0fu, odd = l & 4;
-      const uint32_t got = lane_xor4(odd ? low : high);
-      lo = odd ? got : low;
-      hi = odd ? high : got;
-    }
+    const uint32_t off = (uint32_t)u.first & ((1u << a.shift) - 1), four = off >> 2;
+    const f16 *sc = reinterpret_cast<const f16 *>(blk + ((size_t)D << a.shift) + (size_t)four * (D / 2)) + u.b * 4 + u.tok;
+    kw = *reinterpret_cast<const uint32_t *>(blk + (size_t)(off + u.tok) * (D / 2) + (u.g * NB + u.b) * 4);
+    vw = *reinterpret_cast<const uint32_t *>(blk + ((size_t)(D / 2) << a.shift) + (size_t)four * (2 * D) +
+                                             (l * NB + u.b) * 4);
+    ks = (float)sc[0];
+    vs = (float)sc[4 * NB];
   }
-  if (u.pos < u.s.pos0 || u.pos >= u.s.pos0 + (int32_t)u.s.nrows) return;
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[i] = (float)((int)(lo >> (8 * i) & 0xffu) - 8) * s;
-    x[4 + i] = (float)((int)(hi >> (8 * i) & 0xffu) - 8) * s;
-  }
-  const size_t row = u.s.row0 + (uint32_t)(u.pos - u.s.pos0);
-  store8(u.v ? v + row * ldv + u.col : k + row * ldk + u.col, x);
+  const uint32_t a0 = kw & 0x0f0f0f0fu, a1 = (kw >> 4) & 0x0f0f0f0fu;  // e0 e4 e1 e5, e2 e6 e3 e7
+  if (u.mine)
+    put_row(k + u.row * ldk + u.col, __builtin_amdgcn_perm(a1, a0, 0x06040200u),
+            __builtin_amdgcn_perm(a1, a0, 0x07050301u), ks);
+  vw = transpose4(token_order(vw), l);  // the lane's token of words c = 4 (l >> 2) + 0..3
+  const uint32_t low = vw & 0x0f0f0f0fu, high = (vw >> 4) & 0x0f0f0f0fu, odd = l & 4;
+  const uint32_t got = lane_xor4(odd ? low : high);
+  if (u.mine) put_row(v + u.row * ldv + u.col, odd ? got : low, odd ? high : got, vs);
 }
 
 template <bool STORE, int NB, typename T>
@@ -311,7 +318,7 @@ int run(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, void *k, v
       return fail(MADI_ERR_ARG, "%s: rows of k and v overlap", what);
   }
   // workgroups of 16 units for each four tokens a sequence's rows may touch
-  const uint32_t per_quad = (uint32_t)((2 * width / 32 + 15) / 16);
+  const uint32_t per_quad = (uint32_t)((width / 32 + 15) / 16);
   const uint64_t quads = ((uint64_t)b->rows + 3) / 4 + 1, gx = quads * per_quad;
   if (gx > 0x7fffffffu) return fail(MADI_ERR_SHAPE, "%s: %u rows of %llu elements in one call", what, b->rows,
                                     (unsigned long long)width);
