@@ -551,7 +551,8 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
   a.kv = KV4_GATHER;
   constexpr int P = sizeof(T) == 4 ? 2 : 1;
   constexpr int D = NB * 32;
-  constexpr int R = NB == 2 && W == 4 ? 4 : 2;  // as deep as LDS lets the waves be
+  // as deep as LDS lets the resident waves be; a workgroup alone has few steps per wave
+  constexpr int R = NB == 2 && SHARED ? 4 : 2;
   struct Results {
     float ref[kCols][W], sum[kCols][W], o[W][kCols][D + 4];
   };
