@@ -31,6 +31,7 @@ int kv4_args(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, Kv4Ar
 // extent in bytes.
 int kv4_rows(const char *what, const char *name, const void *p, uint32_t m, uint64_t width,
              uint32_t ld, int dtype, size_t *bytes);
+// Of a cache that kv4_args took.
 inline size_t kv4_cache_bytes(const madi_kv4 *c) {
   return madi_kv4_bytes(c->n_pages, c->page, c->nkv, c->d);
 }
@@ -60,12 +61,13 @@ __device__ inline Kv4Seq kv4_seq(const Kv4Args &a, uint32_t i) {
     lo = kv4_const(a.row_off + i);
     hi = kv4_const(a.row_off + i + 1);
   }
+  // the first row's position by all of the sequence's rows, those past m included
+  const uint32_t all = lo < hi ? hi - lo : 0;
+  s.pos0 = s.len - (int32_t)(all < 0x7fffffffu ? all : 0x7fffffffu);
   hi = hi < a.m ? hi : a.m;
   lo = lo < hi ? lo : hi;
   s.row0 = lo;
-  s.nrows = hi - lo;
-  s.pos0 = s.len - (int32_t)s.nrows;
-  s.nrows = s.nrows < a.rows ? s.nrows : a.rows;
+  s.nrows = hi - lo < a.rows ? hi - lo : a.rows;
   return s;
 }
 // Page of position pos (0 <= pos < reach) of sequence i.

@@ -15,9 +15,10 @@ using namespace madi;
 namespace madi {
 
 namespace {
+// (a page's offsets within a head are 32-bit: 2^20 tokens of 288 bytes)
 bool kv4_shape_ok(uint32_t page, uint32_t nkv, uint32_t d) {
   return (d == 64 || d == 96 || d == 128 || d == 256) && page >= 16 && (page & (page - 1)) == 0 &&
-         page <= (1u << 24) && nkv >= 1 && nkv <= 65535;
+         page <= (1u << 20) && nkv >= 1 && nkv <= 65535;
 }
 }  // namespace
 
@@ -25,9 +26,10 @@ int kv4_args(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, Kv4Ar
   if (!c || !b) return fail(MADI_ERR_NULL, "%s: null pointer", what);
   if (!kv4_shape_ok(c->page, c->nkv, c->d))
     return fail(MADI_ERR_SHAPE,
-                "%s: page %u, nkv %u, d %u (page a power of two from 16 to 2^24, nkv 1 to 65535, d 64, 96, "
+                "%s: page %u, nkv %u, d %u (page a power of two from 16 to 2^20, nkv 1 to 65535, d 64, 96, "
                 "128 or 256)", what, c->page, c->nkv, c->d);
-  if (c->n_pages == 0) return fail(MADI_ERR_SHAPE, "%s: a cache of no pages", what);
+  if (kv4_cache_bytes(c) == 0)
+    return fail(MADI_ERR_SHAPE, "%s: a cache of %u pages (1 to 2^48 bytes)", what, c->n_pages);
   if (b->b > 65535) return fail(MADI_ERR_SHAPE, "%s: %u sequences (at most 65535)", what, b->b);
   if (b->m > 0x7fffffffu || b->rows > 0x7fffffffu)
     return fail(MADI_ERR_SHAPE, "%s: m %u, rows %u (below 2^31)", what, b->m, b->rows);
@@ -62,7 +64,7 @@ int kv4_rows(const char *what, const char *name, const void *p, uint32_t m, uint
   if (dtype != MADI_F16 && dtype != MADI_F32) return fail(MADI_ERR_ARG, "%s: dtype %d", what, dtype);
   if (width > ld) return fail(MADI_ERR_SHAPE, "%s: rows of %s are %u apart but %llu long", what, name, ld,
                               (unsigned long long)width);
-  if (!p) return fail(MADI_ERR_NULL, "%s: null pointer", what);
+  if (!p && m) return fail(MADI_ERR_NULL, "%s: null pointer", what);
   if (!aligned(p, 16) || (uint64_t)ld * es % 16)
     return fail(MADI_ERR_ALIGN, "%s: rows of %s must be 16-byte aligned", what, name);
   if (m) *bytes = ((size_t)(m - 1) * ld + width) * es;
@@ -320,8 +322,8 @@ int run(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, void *k, v
   // workgroups of 16 units for each four tokens a sequence's rows may touch
   const uint32_t per_quad = (uint32_t)((width / 32 + 15) / 16);
   const uint64_t quads = ((uint64_t)b->rows + 3) / 4 + 1, gx = quads * per_quad;
-  if (gx > 0x7fffffffu) return fail(MADI_ERR_SHAPE, "%s: %u rows of %llu elements in one call", what, b->rows,
-                                    (unsigned long long)width);
+  if (gx > 0xffffffu)  // 2^32 threads
+    return fail(MADI_ERR_SHAPE, "%s: %u rows of %llu elements in one call", what, b->rows, (unsigned long long)width);
   if (!initialized()) return fail(MADI_ERR_NOT_INIT, "%s: madi_init has not succeeded", what);
   if (b->m == 0 || b->b == 0 || b->rows == 0) return MADI_OK;
   if (STORE) {
@@ -352,7 +354,8 @@ int run(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, void *k, v
 
 extern "C" size_t madi_kv4_bytes(uint32_t n_pages, uint32_t page, uint32_t nkv, uint32_t d) {
   if (!kv4_shape_ok(page, nkv, d)) return 0;
-  return (size_t)n_pages * nkv * page * (d / 8) * 9;
+  const size_t one = (size_t)nkv * page * (d / 8) * 9;  // below 2^45
+  return n_pages <= ((size_t)1 << 48) / one ? n_pages * one : 0;
 }
 
 extern "C" int madi_kv4_store(const madi_kv4 *cache, const madi_kv4_batch *batch, const void *k,

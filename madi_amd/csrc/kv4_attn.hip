@@ -258,7 +258,6 @@ __device__ inline void make_query(Query<NB, P> &Q, const RawQuery<NB, T> &raw, b
       for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, __builtin_fabsf((float)raw.x[b][e]));
     top = max_across(top);
     k = top > 0 && top < __builtin_inff() ? 11 - __builtin_amdgcn_frexp_expf(top) : 0;
-    k = k < -100 ? -100 : k > 100 ? 100 : k;
   }
   // (never 0, so that it leaves the - infinity of a key not seen what it is)
   Q.fac = __builtin_fmaxf(__builtin_ldexpf(__builtin_fabsf(scale) * 1.4426950408889634f, -k), 1e-37f);
@@ -1172,7 +1171,8 @@ struct Plan {
   size_t bytes() const { return groups ? groups * 2 * part + starts : 0; }
 };
 // A cache of up to four steps per wave stays with one workgroup per tile and head.  Longer ones are dealt out over as many workgroups as are resident at once.
-Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype, uint32_t window, uint32_t cus) {
+Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype, uint32_t window, uint32_t cus,
+             bool most = false) {
   Plan p = {};
   const uint64_t reach = (uint64_t)b->max_pages * c->page;
   uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
@@ -1187,7 +1187,7 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
   const uint64_t cost = (len + 63) / 64 * (prompt_tiles(c->d, dtype == MADI_F32) == 2 ? 5 : 3);
   const uint64_t tiles16 = (cols + kCols - 1) / kCols * c->nkv * b->b;
   const uint64_t rounds = (ptiles * c->nkv * b->b + cus - 1) / cus;
-  if (rounds * cost < tiles16 * steps / (4 * cus)) {
+  if (!most && rounds * cost < tiles16 * steps / (4 * cus)) {
     p.prompt = true;
     p.tiles = (uint32_t)ptiles;
     return p;
@@ -1200,6 +1200,7 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
   if ((len + kKeys - 1) / kKeys <= 4 * waves_alone(c->d, dtype == MADI_F32)) return p;
   // (the row's places are counted in 32 bits)
   if (items * c->nkv * ((reach + kKeys - 1) / kKeys + kOverhead + 1) > 0x40000000u) return p;
+  if (items > 0xfffffu) return p;  // (the join's threads, 4096 per item, likewise)
   p.groups = resident(c->d, dtype == MADI_F32) * cus;
   p.groups = p.groups < kMaxGroups ? p.groups : kMaxGroups;
   return p;
@@ -1237,7 +1238,8 @@ void launch(const AttnArgs &a, const Plan &p, uint32_t cus) {
 extern "C" size_t madi_kv4_attn_bytes(const madi_kv4 *cache, const madi_kv4_batch *batch, uint32_t nh) {
   Kv4Args a;
   if (kv4_args("madi_kv4_attn_bytes", cache, batch, &a) || nh == 0 || nh % cache->nkv) return 0;
-  const Plan p = plan_of(cache, batch, nh, MADI_F16, 0, initialized() ? (uint32_t)cu_count() : 256);
+  // the most that any type and window may take
+  const Plan p = plan_of(cache, batch, nh, MADI_F16, 0, initialized() ? (uint32_t)cu_count() : 256, true);
   return p.bytes();
 }
 
@@ -1272,7 +1274,7 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
   if (p.bytes() > wb) p.groups = wb > p.starts ? (uint32_t)((wb - p.starts) / (2 * p.part)) : 0;
   if (p.groups < 2) p.groups = 0;
   const uint64_t items = (uint64_t)p.tiles * batch->b;
-  if (items * cache->nkv * kCols > 0x7fffffffu)
+  if (items * cache->nkv > 0x3fffffu)  // workgroups of up to 1024 threads, below 2^32 in all
     return fail(MADI_ERR_SHAPE, "%s: %u rows of %u sequences in one call", what, batch->rows, batch->b);
   if (int rc = deferred_before_read(q, qb)) return rc;
   if (int rc = deferred_before_read(cache->data, cb)) return rc;

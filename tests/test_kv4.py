@@ -162,3 +162,36 @@ def test_the_format():
     assert list(s) == [9352, 0] and list(q[:4]) == [7, -7, 0, 7] and not q[4:].any()
     y = np.float32([7, 0.5, -0.5, 1.5, 0.49999997, -2.5] + [0] * 26)
     assert list(R.quantise(y)[0][:6]) == [7, 1, -1, 2, 0, -3]
+
+
+def test_sizes_past_what_an_address_or_a_launch_holds():
+    """Pages of more than 2^20 tokens, caches past 2^48 bytes (their product
+    would wrap) and launches of 2^32 threads are refused."""
+    b = madi_amd.lib().madi_kv4_bytes
+    assert b(1, 1 << 20, 1, 256) == 288 << 20
+    assert b(1, 1 << 21, 1, 64) == 0
+    assert b(0xffffffff, 1 << 20, 65535, 256) == 0 and b(0xffffffff, 16, 1, 64) == 0xffffffff * 16 * 72
+    k, v = FAR + 0x100000, FAR + 0x200000
+    for c in (cache(page=1 << 21), cache(n_pages=0xffffffff, page=1 << 20, nkv=2)):
+        assert call("madi_kv4_store", c, batch(), k, v, 128, 128, 0) == -5
+        assert call("madi_kv4_attn", k, v, c, batch(), 4, 256, 256, 0, 1, 0, 0.125) == -5
+    many = batch(row_off=FAR, rows=0x7fffffff)
+    assert call("madi_kv4_store", cache(nkv=256), many, k, v, 1 << 14, 1 << 14, 0) == -5
+    assert call("madi_kv4_attn", k, v, cache(), many, 4, 256, 256, 0, 1, 0, 0.125) == -5
+    with pytest.raises(madi_amd.MadiError):
+        kv4._bytes(0xffffffff, 1 << 20, 65535, 256)
+
+
+def test_the_workspace_serves_every_type_and_window():
+    """What a batch reserves does not depend on which kernel f16 rows without a
+    window would take: prompts with a window may be split too."""
+    f = lambda b: call("madi_kv4_attn_bytes", cache(nkv=8, d=128), b, 32)
+    one = f(batch(b=1, max_pages=8192, rows=1, m=1))
+    assert f(batch(b=1, max_pages=8192, rows=2048, m=2048)) >= one > 0
+
+
+def test_a_call_without_rows():
+    """No rows: no row pointers are needed (torch gives an empty tensor none)."""
+    b = batch(b=0, m=0)
+    assert call("madi_kv4_store", cache(), b, None, None, 128, 128, 0) == -8  # (madi_init, as for any other call)
+    assert call("madi_kv4_attn", None, None, cache(), b, 4, 256, 256, 0, 1, 0, 0.125) == -8
