@@ -355,7 +355,8 @@ template <int NB>
 __device__ inline void cut_scales(Step<NB> &t, int32_t key, int32_t len, uint32_t r, uint32_t g) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int32_t k = key + 16 * i + 4 * (int32_t)g + 2 * (int32_t)(r & 1);
+    // (lanes past the words hold the last one, of tokens 2 and 3)
+    const int32_t k = key + 16 * i + 4 * (int32_t)g + (r >= 4 * NB ? 2 : 2 * (int32_t)(r & 1));
     uint32_t keep = t.there[i] && k < len ? 0xffffu : 0;
     if (t.there[i] && k + 1 < len) keep |= 0xffff0000u;
 #pragma unroll

@@ -271,3 +271,24 @@ def test_two_streams_and_two_graphs_at_once(kv4):
     finally:
         torch.cuda.synchronize()
         q8.init()
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_large_scales_past_the_end(kv4, d, dtype):
+    """The pool's other scales are the largest finite f16 numbers: what a
+    sequence does not hold has no part in the exponent that its V scales share
+    (with it, P would lose up to 16 bits), wherever in four tokens it ends."""
+    say(f"large scales past the end {d} {dtype}")
+    rng = np.random.default_rng(27)
+    s = Setup(kv4, rng, 2, d, 16, [1, 18, 31, 44, 61], [1] * 5)
+    s.data[..., 0::2], s.data[..., 1::2] = 0xff, 0x7b
+    s.fill(rng)
+    q = queries(rng, s, 4, dtype)
+    want, tol = s.expect(q, 4, True, 0, d ** -0.5, dtype)
+    got = attend(s, q, 4, dtype)
+    for i in range(5):
+        # (each row's own error: a single sequence's would be small beside the others)
+        err = np.linalg.norm((got - want)[i]) / np.linalg.norm(want[i])
+        assert err <= (5e-6 if dtype == "f32" else 2e-3), (i, err)
+    check(got, want, tol, dtype)
