@@ -222,9 +222,11 @@ __device__ inline void read_step(Step<NB> &t, const uint8_t *slot, uint32_t ther
 // The wave's state for its 16 columns.
 template <int NB>
 struct Acc {
-  f32x4 o[2 * NB];  // O^T tiles, scaled like P
-  float ref, sum;   // M, and this lane's part of sum P
-  float down, most; // 2^-e, and the largest V scale that it serves
+  f32x4 o[2 * NB];     // O^T tiles, scaled like P
+  float ref, sum;      // M + e, and this lane's part of the sum of P 2^-e
+  float limit;         // M + kRaise
+  float e, most;       // the column's e, and the largest V scale that it serves
+  float check;         // lanes of V scales: the least `most` of all columns; else infinity
 };
 
 // Q^T as B operands, P parts per block.
@@ -402,21 +404,47 @@ __device__ inline void rescale(Acc<NB> &A, float f) {
     for (int j = 0; j < 4; ++j) A.o[n][j] *= f;
 }
 
+// A larger score or V scale than M and e serve: new ones, per column.  `big` is
+// the lane's largest V scale, of which in a step that all columns see whole
+// each is any column's; else a column takes those of the keys it sees (a key that
+// a row does not see, an infinity's maybe, costs its P no bits).
+template <int NB>
+__device__ inline void raise(Acc<NB> &A, const VScales<NB> &c, const float (&x)[8], float top, float big, bool whole) {
+  const bool mine = (threadIdx.x & 15) >= VScales<NB>::kLane;
+  if (whole) {
+    big = wave_max(mine ? big : 0.0f);
+  } else {
+    big = 0;
+    each<2>([&](auto I) {
+      each<4 * NB>([&](auto N) {
+        constexpr int i = I(), n = N();
+        const float s = c.template of<n>(i);
+        big = __builtin_fmaxf(big, x[4 * i + n % 4] > -__builtin_inff() ? s : 0.0f);
+      });
+    });
+    big = max_across(big);
+  }
+  top = max_across(top);
+  // the reference of a column that has seen no key stays
+  if (top > A.limit) A.limit = top - kLift + kRaise;
+  if (big > A.most) {
+    const int e = __builtin_amdgcn_frexp_expf(big);
+    A.e = (float)e;
+    A.most = __builtin_ldexpf(2.0f, e);
+  }
+  const float ref = A.limit - kRaise + A.e, f = __builtin_amdgcn_exp2f(A.ref - ref);
+  A.ref = ref;
+  A.sum *= f;
+  rescale(A, f);
+  A.check = mine ? -wave_max(-A.most) : __builtin_inff();
+}
+
 // Softmax weights of a step and their product with V.
 template <int NB, int P>
-__device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const Step<NB> &t, const Masks &m) {
+__device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const Step<NB> &t, const Masks &m, bool whole) {
   float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3])),
                               __builtin_fmaxf(__builtin_fmaxf(x[4], x[5]), __builtin_fmaxf(x[6], x[7])));
   top *= fac;
-  if (__any(top > A.ref + kRaise)) {
-    top = max_across(top);
-    // the reference of a column that has seen no key stays
-    const float ref = top > A.ref + kRaise ? top - kLift : A.ref;
-    const float f = __builtin_amdgcn_exp2f(A.ref - ref);
-    A.ref = ref;
-    A.sum *= f;
-    rescale(A, f);
-  }
   VScales<NB> c;
   float big = 0;
 #pragma unroll
@@ -428,25 +456,12 @@ __device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const St
       c.s[i][n][1] = (float)w.y;
       big = __builtin_fmaxf(big, __builtin_fmaxf(c.s[i][n][0], c.s[i][n][1]));
     }
-  if (__any(big > A.most)) {  // (a lane of K scales has an infinite `most`)
-    const bool mine = (threadIdx.x & 15) >= VScales<NB>::kLane;
-    big = wave_max(mine ? big : 0.0f);
-    const float down = __builtin_ldexpf(1.0f, -__builtin_amdgcn_frexp_expf(big));
-    rescale(A, down / A.down);
-    A.down = down;
-    A.most = mine ? 2 / down : __builtin_inff();
-  }
+  if (__any(top > A.limit || big > A.check)) raise<NB>(A, c, x, top, big, whole);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], fac, -A.ref));
     A.sum += x[i];
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int n = VScales<NB>::kFirst; n < Step<NB>::kScaleWords; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) c.s[i][n][h] *= A.down;
   each<NB>([&](auto B) {
     constexpr int b = B();
     uint32_t ph[4], pl[4];
@@ -690,8 +705,9 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
       Acc<NB> A;
       A.ref = kNever;
       A.sum = 0;
-      A.down = 1;
-      A.most = r >= 2 * NB % 16 ? 0.0f : __builtin_inff();
+      A.limit = kNever;
+      A.e = A.most = 0;
+      A.check = r >= VScales<NB>::kLane ? 0.0f : __builtin_inff();
 #pragma unroll
       for (int n = 0; n < 2 * NB; ++n) A.o[n] = (f32x4){0, 0, 0, 0};
 
@@ -713,7 +729,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
         float x[8];
         scores<NB, P>(x, Q, st);
         if (!whole) cut_scores<NB>(x, st, key, lo, hi, g);
-        add_values<NB, P>(A, x, Q.fac, st, m);
+        add_values<NB, P>(A, x, Q.fac, st, m, whole);
         at += W;
       }
       A.sum = sum_across(A.sum);
@@ -724,7 +740,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
       float ref = kNever;
 #pragma unroll
       for (int w = 0; w < W; ++w) ref = __builtin_fmaxf(ref, res.ref[r][w]);
-      const float f = __builtin_amdgcn_exp2f(A.ref - ref), fo = f / (A.down * kCodeUnit);  // (f times a power of two)
+      const float f = __builtin_amdgcn_exp2f(A.ref - ref), fo = f / kCodeUnit;
       if (g == 0) res.sum[r][wave] = A.sum * f;
       if (mine)
 #pragma unroll

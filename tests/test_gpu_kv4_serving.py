@@ -292,3 +292,40 @@ def test_large_scales_past_the_end(kv4, d, dtype):
         err = np.linalg.norm((got - want)[i]) / np.linalg.norm(want[i])
         assert err <= (5e-6 if dtype == "f32" else 2e-3), (i, err)
     check(got, want, tol, dtype)
+
+
+@pytest.mark.parametrize("heads,group,d,lens,rows,window", [
+    (2, 2, 64, [60, 37], [9, 5], 0), (1, 4, 128, [90, 133], [20, 40], 24), (2, 1, 96, [2500, 40], [3, 2], 0),
+    (1, 2, 256, [50, 17], [16, 3], 8), (16, 16, 64, [230, 233], [230, 190], 40), (16, 16, 128, [250, 230], [230, 230], 0),
+])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_infinities_that_a_row_does_not_see(kv4, heads, group, d, lens, rows, window, dtype):
+    """K and V of each sequence's last token, and of one that all windows have
+    passed, hold infinities and NaN: rows that do not see them lose nothing."""
+    say(f"infinities {heads}x{group}x{d} {lens} {rows} window {window} {dtype}")
+    rng = np.random.default_rng(28)
+    s = Stored(kv4, rng, heads, d, 16, lens, rows)
+    s.fill(rng)
+    spots = [(i, n - 1) for i, n in enumerate(lens)]
+    if window:
+        spots += [(i, n - rows[i] - window) for i, n in enumerate(lens) if n - rows[i] - window >= 0]
+    for i, pos in spots:
+        x = rng.standard_normal((1, 2, heads, d)).astype(np.float32)
+        x[..., ::5], x[..., 1::7], x[..., 2::9] = np.inf, -np.inf, np.nan
+        one = kv4.Batch(s.batch.table[i:i + 1], torch.tensor([pos + 1], dtype=torch.int32).cuda(), rows=1)
+        kv = torch.from_numpy(x).cuda()
+        kv4.kvStore(s.cache, one, kv[:, 0], kv[:, 1])
+        torch.cuda.synchronize()
+        for held, new in zip(s.held[i], (*R.quantise(x[:, 0]), *R.quantise(x[:, 1]))):
+            held[pos] = new[0]
+    nh = heads * group
+    q = queries(rng, s, nh, dtype)
+    want, tol = s.expect(q, nh, True, window, d ** -0.5, dtype)
+    got = attend(s, q, nh, dtype, True, window)
+    unseen = [s.off[i] + r for i, n in enumerate(lens) for r, pos in enumerate(R.rows_of(n, rows[i])) if pos < n - 1]
+    err = np.linalg.norm((got - want)[unseen], axis=-1) / np.maximum(np.linalg.norm(want[unseen], axis=-1), 1e-3)
+    say(f"  worst row {err.max():.2e}")
+    # (a row's own error: for f32 rows its scores' and the 22 bits of q and P, for f16 rows two roundings)
+    assert err.max() <= (2e-5 if dtype == "f32" else 2e-3)
+    seen = [r for r in range(s.m) if r not in unseen]
+    assert np.all(np.abs(got - want)[seen] <= tol[seen])
