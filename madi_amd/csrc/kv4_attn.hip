@@ -436,7 +436,8 @@ __device__ inline void raise(Acc<NB> &A, const VScales<NB> &c, const float (&x)[
   A.ref = ref;
   A.sum *= f;
   rescale(A, f);
-  A.check = mine ? -wave_max(-A.most) : __builtin_inff();
+  const float least = -wave_max(-A.most);  // (with all lanes active: not inside the ?:)
+  A.check = mine ? least : __builtin_inff();
 }
 
 // Softmax weights of a step and their product with V.
@@ -681,6 +682,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
         if (issued < end) {
           if (next == kListed) {
             listed = list_pages(a.kv, t.seq, (uint32_t)(t.first + issued), W, lane);
+            asm volatile("" : "+v"(listed));  // (waited for here, not, with all loads of the ring, at each step)
             next = 0;
           }
           const uint32_t pages[2] = {(uint32_t)__builtin_amdgcn_readlane(listed, 2 * next),
@@ -696,6 +698,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
       // (the queries are asked for first: theirs is the shorter way)
       const RawQuery<NB, T> raw(static_cast<const T *>(a.q) + (size_t)(s.row0 + row) * a.ldq +
                                 (size_t)(head * a.group + sub) * D + 8 * g);
+      asm volatile("" : "+v"(listed));
 #pragma unroll 1
       for (int n = 0; n < R - 1; ++n) issue();
 
