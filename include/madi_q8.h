@@ -360,8 +360,9 @@ int madi_flash_enc_f16(void *out, const void *q, const void *k, const void *v, u
  *          (high nibbles), its bytes tokens 4u, 4u+2, 4u+1, 4u+3
  *   scales page * d/8 bytes: tokens 4u..4u+3 at u * d/2; f16 (x, b, t) at
  *          ((x * nb + b) * 4 + t) * 2, x = 0 for K and 1 for V, t the token - 4u
- * d is 64, 96, 128 or 256; page a power of two, at least 16; data 16-byte
- * aligned.  madi_kv4_bytes gives the size of data (0 for a shape it does not take). */
+ * d is 64, 96, 128 or 256; page a power of two from 16 to 2^20; data 16-byte
+ * aligned, 2^48 bytes at most.  madi_kv4_bytes gives the size of data (0 for a
+ * shape it does not take). */
 typedef struct {
   void *data;       /* device */
   uint32_t n_pages; /* pages in the pool */
@@ -414,9 +415,13 @@ int madi_kv4_load(void *k, void *v, uint32_t ldk, uint32_t ldv, int dtype, const
  * head, q and out [m][nh * d] (rows ldq and ldo elements apart, 16-byte
  * aligned).  causal: the row at position p sees positions j <= p and, where window
  * is not 0, j > p - window; not causal (cross-attention): all lens[i] of them,
- * window 0.  A row that sees no key becomes zeros.  Scores, softmax and sums
- * are f32.  With f16 rows the probabilities and V values enter the product as
- * f16; with f32 rows every operand is kept to 22 bits or more.  out may be q
+ * window 0.  A row that sees no key becomes zeros; a key that a row does not
+ * see leaves no trace in it, whatever it holds.  Scores, softmax and sums are
+ * f32.  With f16 rows a probability enters the product as one f16, times its
+ * V scale (single tokens and short prompts) or by itself (long prompts);
+ * K and V enter exactly (long prompts: V below 2^-14 to 2^-25).  With f32
+ * rows every operand is kept to 22 bits or more of the largest that its row
+ * sees; q may be of any magnitude.  out may be q
  * itself (same rows), else it must not overlap it. */
 int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, const madi_kv4_batch *batch,
                   uint32_t nh, uint32_t ldo, uint32_t ldq, uint32_t window, int causal, int dtype,

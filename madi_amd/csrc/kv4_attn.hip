@@ -9,17 +9,31 @@
 //     block's sum gets its key's scale in f32: S = sum_b s_b (Q K^T)_b.  (Codes
 //     masked into f16 subnormals would need no bias taken off, but the matrix
 //     core sums products of subnormals to 2^-18 only, against 2^-24.)
-//   softmax over a running reference that is raised only when a score passes
-//     it by 2^8, so most steps exchange nothing between lanes.
+//   softmax over a running reference M that is raised only when a score passes the
+//     largest at its last raise by 2^7 (in the exponents of 2), so most steps
+//     exchange nothing between lanes.
 //   O^T += V^T P^T, 32 keys as K and 16 elements as rows: P^T comes straight
 //     from the S^T registers (lane (g, c) holds keys 4g..4g+3 of both tiles),
 //     V as its codes from the words that hold four tokens, and the V scale of a
 //     key and block goes into P: one rounding, of P s, instead of P's and V's.
-//     s comes times 2^-e, e the largest exponent among the wave's V scales so
-//     far, so that P s stays within f16.
+//     P comes times 2^-e, e the exponent of the largest V scale that the column
+//     has seen, so that P s stays within f16: 2^-e is part of the reference
+//     M + e and costs nothing.
 // A lane holds two of the 8 nb scales of its four keys and passes them to the
 // other 15 through DPP broadcasts, which cost nothing in a multiplication.
 // f32 rows: q and P s are each split in two f16 (22 bits).
+//
+// What it costs (us, f16 rows, d 128; one MI355X):
+//   128 sequences of 8192, 32 heads over 8: 229, 1.21 GB at 5.3 TB/s of the 6.5
+//     that a kernel which only reads reaches.  A step of 32 keys is 326 vector
+//     instructions (144 make codes of nibbles, 48 apply the K scales, 48 make P s)
+//     and 16 MFMAs: the vector pipe is busy 70 % of the time, the matrix pipe 14 %,
+//     and 16 % of the waves' time is waiting for memory or barriers.
+//   1 sequence of 131072: 40.6, 33 in the kernel (4.6 TB/s; eight steps per wave
+//     do not hide a segment's beginning and end), 5.4 in the join.
+//   1 token over 213 keys, 20 heads of 64, f32: 5.7, of which 3 are launch and
+//     the rest five dependent memory latencies (length, pages, words, results in
+//     LDS, store).
 #include <type_traits>
 
 #include "kv4.h"
@@ -39,11 +53,13 @@ constexpr int prompt_keys(int d) { return d == 256 ? 32 : 64; }
 constexpr float kNever = -1e30f;  // reference before any key was seen
 // P is 2^(x - M) with M at first the largest x - 7, raised when an x passes M
 // by 14: P at most 2^14, P s 2^-e at most 2^15 (f16 holds 2^16), and what
-// rounds to nothing is 2^-32 of the largest P at the largest s.
+// rounds to nothing is 2^-32 of the largest P at the largest s.  (A reference that
+// follows the largest score at each step would rescale 32 registers each time.)
 constexpr float kLift = 7.0f, kRaise = 14.0f;
 
 // What a segment costs beside its steps (finding it, its queries, the first
-// words' latency, the waves' results put together), in steps.
+// words' latency, the waves' results put together), in steps.  (4, 8, 12 and 16 were
+// timed on 48 ragged sequences and on 128 of 8192: 8 and 12 are the best of both.)
 constexpr uint32_t kOverhead = 8;
 // Workgroups that share the steps, at most.
 constexpr uint32_t kMaxGroups = 1024;
@@ -55,9 +71,10 @@ constexpr size_t kShare = kCols * (D + 2);
 // the low parts) and by LDS (the ring).
 constexpr uint32_t resident(uint32_t d, bool f32) { return d == 256 ? 2 : f32 && d == 128 ? 3 : 4; }
 
-// Waves of a workgroup that has a tile and head for itself: as many as fit a CU's
-// registers.
+// Waves of a workgroup that has a tile and head for itself and more than kFew steps:
+// as many as fit a CU's registers.
 constexpr uint32_t waves_alone(uint32_t d, bool f32) { return 4 * resident(d, f32) > 12 ? 16 : 8; }
+constexpr uint32_t kFew = 8;
 
 struct AttnArgs {
   Kv4Args kv;
@@ -137,7 +154,7 @@ struct Step {
 
 // Page numbers of the wave's next kListed steps, two per step, one per lane: `at`
 // is the first step, the others come `stride` apart.  (A scalar load per step
-// would be waited for with the step's LDS reads.)
+// would be waited for with the step's LDS reads.)  Past the table's end any entry stands in.
 constexpr int kListed = 32;
 __device__ inline uint32_t list_pages(const Kv4Args &a, uint32_t seq, uint32_t at, uint32_t stride, uint32_t lane) {
   const uint32_t n = ((at + (lane >> 1) * stride) * kKeys + (lane & 1) * 16) >> a.shift;
@@ -562,6 +579,11 @@ __device__ inline uint32_t wave_scan(uint32_t v) {
 // for kv4_attn_join_kernel.  A workgroup has two places there: 0 for
 // a segment that others began, 1 for one that it begins and does not end.
 // Else: a workgroup per item and head.
+//
+// Dealt out because lengths differ and heads are few: 48 sequences of 1 to 8000
+// tokens take 23.6 us with the join, 45.9 with a workgroup per item and head,
+// one of 131072 40.6 and 665; 128 equal ones of 8192, 1024 items and heads, 229 and 228.
+// With a workgroup alone there is no second launch (a join is 4.5 to 6 us).
 template <int NB, int W, bool SHARED, typename T>
 __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4_attn_kernel(KV4_PARAMS, AttnArgs a) {
   a.kv = KV4_GATHER;
@@ -736,7 +758,7 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
         at += W;
       }
       A.sum = sum_across(A.sum);
-          // the waves' results: brought to a common reference, then added up
+      // the waves' results: brought to a common reference, then added up
       __syncthreads();
       if (g == 0) res.ref[r][wave] = A.ref;
       __syncthreads();
@@ -781,6 +803,8 @@ __global__ __launch_bounds__(64 * W, resident(NB * 32, sizeof(T) == 4)) void kv4
 // The segments of one column of an item and head, joined, where there are more
 // than one: a workgroup per item and column, and head.  The segments' weights
 // first, then D threads add up their O, TH / D groups of them every so many segments.
+// Bound by two dependent memory latencies and the launch: 5.4 us for 128
+// segments of 32 columns, 5.9 for two or three of 4096.
 template <int NB, int TH, typename T>
 __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(KV4_PARAMS, AttnArgs a, uint32_t tile_cols) {
   a.kv = KV4_GATHER;
@@ -849,7 +873,12 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(KV4_PARAMS, AttnArgs 
 //   V as (n - 8) s in two f16, which hold all of its 15 bits: rounded to one
 //     it would add an error like P's own rounding, and so would K.
 // For 64 keys and 16 columns at d 128 that is 48 MFMAs (768 cycles) and about 200
-// vector instructions (800 cycles), against 64 scores per lane group.
+// vector instructions (800 cycles), which do not run beside each other in one
+// wave, and the two waves of a SIMD meet at a barrier each 64 keys.  2048 rows
+// over 16384 keys (causal, 32 heads of 128 over 8): 748 us, 689 TFLOP/s of the
+// product's 2 x 2 operations, the high and low V's third MFMA not counted (a
+// library f16 product of 8192^3 reaches 1168).  Two groups of waves, one multiplying while the other
+// does its softmax, took 860: each then has half of the registers' reuse of an operand.
 template <int NB, int KC>
 struct Buffer {
   static constexpr int kTiles = KC / 16;
@@ -1162,7 +1191,6 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PA
       if (st == Wd::kBlocks) fetch(c + 2);
     }
     __builtin_amdgcn_sched_barrier(0);
-    
     } else {
       put_all(c + 1);
       fetch(c + 2);
@@ -1184,13 +1212,18 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PA
 
 struct Plan {
   uint32_t tiles, groups;  // groups: workgroups that share the steps, 0: one per tile and head
-  bool few;                // steps (up to eight)
+  bool few;                // steps
   bool prompt;
   size_t part;             // bytes of a partial result
   size_t starts;           // bytes of the items' starts
   size_t bytes() const { return groups ? groups * 2 * part + starts : 0; }
 };
-// A cache of up to four steps per wave stays with one workgroup per tile and head.  Longer ones are dealt out over as many workgroups as are resident at once.
+// A cache of up to four steps per wave (2048 keys at d 64) stays with one workgroup
+// per tile and head: eight sequences of 1500, 20 heads of 64, f32, take 13.1 us
+// there and 16.7 dealt out and joined; from more steps per wave on the join is the
+// smaller part.  Longer ones are dealt out over as many workgroups as are
+// resident at once.  most: without the prompts' kernel, whose place
+// depends on the type and window.
 Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype, uint32_t window, uint32_t cus,
              bool most = false) {
   Plan p = {};
@@ -1198,10 +1231,11 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
   uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
   if (window && (uint64_t)window + b->rows + kKeys < len) len = (uint64_t)window + b->rows + kKeys;
   const uint64_t cols = (uint64_t)b->rows * (nh / c->nkv);
-  // Prompts where their workgroups fill the device: one of them takes as long for
+  // Prompts where their workgroups fill the device.  One of them takes as long for
   // 64 keys as a wave of the other kernel, of which a CU has 16 (four times as fast
-  // as one), for 5 * 4 of its steps with two tiles of columns per wave, 3 * 4 with one.  (2048 rows over 16384 keys, 8 x 4 heads of 128: 744 us here, 1250 there; four of 224 rows
-  // over as many keys, 20 heads of 64, f32: 17 us here, 10 there.)
+  // as one), for 5 * 4 of its steps with two tiles of columns per wave, 3 * 4 with
+  // one.  (2048 rows over 16384 keys, 32 heads of 128 over 8: 748 us here, 1411
+  // there; four of 17 to 224 rows over as many keys, 20 heads of 64, f32: 17.3 us here, 9.8 there.)
   const uint64_t pcols = (uint64_t)kPromptWaves * 16 * prompt_tiles(c->d, dtype == MADI_F32);
   const uint64_t ptiles = (cols + pcols - 1) / pcols, steps = (len + kKeys - 1) / kKeys;
   const uint64_t cost = (len + 63) / 64 * (prompt_tiles(c->d, dtype == MADI_F32) == 2 ? 5 : 3);
@@ -1216,7 +1250,7 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
   p.part = (size_t)kCols * (c->d + 2) * 4;
   const uint64_t items = (uint64_t)p.tiles * b->b;
   p.starts = (size_t)(items + 1) * 4;
-  p.few = (len + kKeys - 1) / kKeys <= 8;
+  p.few = (len + kKeys - 1) / kKeys <= kFew;
   if ((len + kKeys - 1) / kKeys <= 4 * waves_alone(c->d, dtype == MADI_F32)) return p;
   // (the row's places are counted in 32 bits)
   if (items * c->nkv * ((reach + kKeys - 1) / kKeys + kOverhead + 1) > 0x40000000u) return p;
@@ -1234,11 +1268,9 @@ void launch(const AttnArgs &a, const Plan &p, uint32_t cus) {
   }
   if (!p.groups) {
     constexpr int W = waves_alone(NB * 32, sizeof(T) == 4);
-    // few steps: a wave each while a workgroup has a CU for itself, else four waves
-    if (p.few && a.items * a.kv.nkv <= 2 * cus)
-      kv4_attn_kernel<NB, 8, false, T><<<a.items * a.kv.nkv, 512, 0, stream()>>>(KV4_ARGS(a.kv), a);
-    else if (p.few)
-      kv4_attn_kernel<NB, 4, false, T><<<a.items * a.kv.nkv, 256, 0, stream()>>>(KV4_ARGS(a.kv), a);
+    // few steps: four waves (20 heads over 213 keys 5.7 us, with eight 5.95, with
+    // sixteen 6.7; prompts of 17 to 224 rows, four of them, 9.8, 11.0 and 19.2)
+    if (p.few) kv4_attn_kernel<NB, 4, false, T><<<a.items * a.kv.nkv, 256, 0, stream()>>>(KV4_ARGS(a.kv), a);
     else kv4_attn_kernel<NB, W, false, T><<<a.items * a.kv.nkv, 64 * W, 0, stream()>>>(KV4_ARGS(a.kv), a);
     return;
   }
@@ -1246,7 +1278,9 @@ void launch(const AttnArgs &a, const Plan &p, uint32_t cus) {
   const uint64_t cols = (uint64_t)a.kv.rows * a.group;
   const uint32_t tile_cols = cols < kCols ? (uint32_t)cols : kCols;
   const dim3 grid(a.items * tile_cols, a.kv.nkv);
-  // few columns are of long caches, many segments each; of many most have one
+  // few columns are of long caches, many segments each: 131072 keys, 32 columns,
+  // 40.6 us with 1024 threads, 43.7 with 256.  Of many most have one or two: 128
+  // sequences of 8192 229 us with 256 threads, 240 with 1024; 48 ragged ones 23.6, 29.3.
   if ((uint64_t)grid.x * grid.y <= 2 * cus)
     kv4_attn_join_kernel<NB, 1024, T><<<grid, 1024, 0, stream()>>>(KV4_ARGS(a.kv), a, tile_cols);
   else
