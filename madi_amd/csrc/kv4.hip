@@ -6,8 +6,16 @@
 // that a V word (four tokens' bytes) is made in one place.  Lane l of the 16 has
 // token l & 3 and elements 32b + 8g .. + 7, g = 2 (l >> 2 & 1) + (l >> 3): with
 // this order the V words come out of two byte transposes between neighbouring lanes
-// (DPP) instead of through LDS.  Both are bound by memory: K's and V's loads are
-// in flight together.
+// (DPP) instead of through LDS.  A border between two codes costs one
+// multiply-add beside the estimate (see code()), no division.
+//
+// Both are bound by memory, K's and V's loads in flight together: 131072 rows
+// of 8 heads of 128 in f16 read back in 137 us (0.69 GB at 5.0 TB/s, where a copy
+// reaches 4.7: three quarters are writes), 16384 stored in 28.8 (3.0 TB/s: the codes'
+// arithmetic, about as long as the copy, is not all hidden behind it) and read back in
+// 15.2, single rows of eight sequences in 3.8 and 2.8, which is the latencies of a
+// length, a page number and the rows, one after the other.  (Two units per lane: 130
+// us for the first, but 24 sequences' ragged prompts 17.8 in place of 13.8, stored and read.)
 #include "kv4.h"
 
 using namespace madi;
@@ -109,8 +117,8 @@ __device__ inline void load8(const f16 *p, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
 }
-// (not kept in the L2, which the rows mostly exceed: 131072 rows of 8 heads of 128 read
-// back in 173 us, 184 with ordinary stores)
+// (not kept in the L2, which the rows mostly exceed: with ordinary stores 131072 rows of 8
+// heads of 128 took 6 % longer to read back)
 __device__ inline void store8(float *p, const float (&x)[8]) {
   __builtin_nontemporal_store((f32x4){x[0], x[1], x[2], x[3]}, reinterpret_cast<f32x4 *>(p));
   __builtin_nontemporal_store((f32x4){x[4], x[5], x[6], x[7]}, reinterpret_cast<f32x4 *>(p + 4));
@@ -319,7 +327,8 @@ int run(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, void *k, v
     if (ldk != ldv || gap < w || row - gap < w)
       return fail(MADI_ERR_ARG, "%s: rows of k and v overlap", what);
   }
-  // workgroups of 16 units for each four tokens a sequence's rows may touch
+  // workgroups of 16 units for each four tokens a sequence's rows may touch (those of
+  // shorter sequences end at once)
   const uint32_t per_quad = (uint32_t)((width / 32 + 15) / 16);
   const uint64_t quads = ((uint64_t)b->rows + 3) / 4 + 1, gx = quads * per_quad;
   if (gx > 0xffffffu)  // 2^32 threads

@@ -869,7 +869,7 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(KV4_PARAMS, AttnArgs 
 // next KC keys' operands go to LDS while these are multiplied (two buffers, one
 // barrier per KC keys), the words of the ones after that are on their way in
 // registers.  The operands lie in LDS as the MFMAs read them, 16 bytes per lane.
-//   K as its codes (the block sums get their scales, f16 in LDS, afterwards);
+//   K as its codes (the block sums get their scales, f32 in LDS, afterwards);
 //   V as (n - 8) s in two f16, which hold all of its 15 bits: rounded to one
 //     it would add an error like P's own rounding, and so would K.
 // For 64 keys and 16 columns at d 128 that is 48 MFMAs (768 cycles) and about 200
@@ -877,8 +877,8 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(KV4_PARAMS, AttnArgs 
 // wave, and the two waves of a SIMD meet at a barrier each 64 keys.  2048 rows
 // over 16384 keys (causal, 32 heads of 128 over 8): 748 us, 689 TFLOP/s of the
 // product's 2 x 2 operations, the high and low V's third MFMA not counted (a
-// library f16 product of 8192^3 reaches 1168).  Two groups of waves, one multiplying while the other
-// does its softmax, took 860: each then has half of the registers' reuse of an operand.
+// library f16 product of 8192^3 reaches 1168).  Two groups of waves, one multiplying while the
+// other does its softmax, took 860.
 template <int NB, int KC>
 struct Buffer {
   static constexpr int kTiles = KC / 16;
