@@ -11,9 +11,9 @@
 //
 // Both are bound by memory, K's and V's loads in flight together: 131072 rows
 // of 8 heads of 128 in f16 read back in 137 us (0.69 GB at 5.0 TB/s, where a copy
-// reaches 4.7: three quarters are writes), 16384 stored in 28.8 (3.0 TB/s: the codes'
-// arithmetic, about as long as the copy, is not all hidden behind it) and read back in
-// 15.2, single rows of eight sequences in 3.8 and 2.8, which is the latencies of a
+// reaches 4.7: three quarters are writes), 16384 stored in 23.4 (3.7 TB/s: the codes'
+// arithmetic is not all hidden behind the copy) and read back in
+// 15.4, single rows of eight sequences in 3.6 and 2.9, which is the latencies of a
 // length, a page number and the rows, one after the other.  (Two units per lane: 130
 // us for the first, but 24 sequences' ragged prompts 17.8 in place of 13.8, stored and read.)
 #include "kv4.h"
@@ -130,18 +130,18 @@ __device__ inline void store8(f16 *p, const float (&x)[8]) {
   __builtin_nontemporal_store(v, reinterpret_cast<f16x8 *>(p));
 }
 
-// The code of x (plus 8) against scale s > 0: |x| / s to the nearest whole
-// number, halves away from zero.  rcp's estimate is off by less than one
-// near a border; the remainder a - q s is exact there (s has 11 bits and q 4),
-// so comparing it with s / 2, exact too, settles the code.
-__device__ inline uint32_t code(float x, float s, float inv, float half) {
+// The code of x plus 8, as a number, against scale s > 0: |x| / s to the nearest
+// whole number, halves away from zero.  `inv` is 1 / s taken 2^-21 too small, more than
+// rcp and the multiply-add are off (by 2^-23 and 2^-24 of |x| / s + 1/2), so the estimate
+// is the code or one less.  The remainder a - q s is exact in f32 (s has 11 bits and
+// q 4), so comparing it with s / 2, exact too, settles the code.  A NaN's is 0: the
+// maximum drops it, and it compares with nothing.
+constexpr float kBelow = 1 - 0x1p-21f;
+__device__ inline float code(float x, float s, float inv, float half) {
   const float a = __builtin_fabsf(x);
-  float q = __builtin_fminf(__builtin_floorf(__builtin_fmaf(a, inv, 0.5f)), 7.0f);
-  const float r = __builtin_fmaf(-q, s, a);
-  q += r >= half ? 1.0f : 0.0f;
-  q -= r < -half ? 1.0f : 0.0f;
-  q = __builtin_fminf(q, 7.0f);
-  return (uint32_t)(8 + (int)__builtin_copysignf(q, x));
+  float q = __builtin_fminf(__builtin_fmaxf(__builtin_floorf(__builtin_fmaf(a, inv, 0.5f)), 0.0f), 7.0f);
+  q += __builtin_fmaf(-q, s, a) >= half ? 1.0f : 0.0f;
+  return 8.0f + __builtin_copysignf(__builtin_fminf(q, 7.0f), x);
 }
 
 struct Unit {
@@ -173,12 +173,11 @@ __device__ inline bool unit_of(const Kv4Args &a, uint32_t per_quad, Unit &u) {
 }
 
 // The codes (plus 8, a byte each) of the lane's 8 elements and their block's scale.
-__device__ inline f16 quantise(float (&x)[8], uint32_t &lo, uint32_t &hi) {
+__device__ inline f16 quantise(const float (&x)[8], uint32_t &lo, uint32_t &hi) {
   float top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    x[i] = x[i] == x[i] ? x[i] : 0.0f;  // a NaN is held as 0
-    top = __builtin_fmaxf(top, __builtin_fabsf(x[i]));
+    top = __builtin_fmaxf(top, __builtin_fabsf(x[i]));  // (of a NaN and a number the number)
   }
   // the four lanes of the token's block
   top = __builtin_fmaxf(top, __builtin_bit_cast(float, dpp<kRor4>(__builtin_bit_cast(uint32_t, top))));
@@ -188,12 +187,11 @@ __device__ inline f16 quantise(float (&x)[8], uint32_t &lo, uint32_t &hi) {
   const float s = (float)sh;
   lo = hi = 0x08080808u;
   if (s > 0) {
-    const float inv = __builtin_amdgcn_rcpf(s), half = 0.5f * s;
-    lo = hi = 0;
+    const float inv = __builtin_amdgcn_rcpf(s) * kBelow, half = 0.5f * s;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      lo |= code(x[i], s, inv, half) << (8 * i);
-      hi |= code(x[4 + i], s, inv, half) << (8 * i);
+      lo = __builtin_amdgcn_cvt_pk_u8_f32(code(x[i], s, inv, half), i, lo);
+      hi = __builtin_amdgcn_cvt_pk_u8_f32(code(x[4 + i], s, inv, half), i, hi);
     }
   }
   return sh;
