@@ -329,3 +329,29 @@ def test_infinities_that_a_row_does_not_see(kv4, heads, group, d, lens, rows, wi
     assert err.max() <= (2e-5 if dtype == "f32" else 2e-3)
     seen = [r for r in range(s.m) if r not in unseen]
     assert np.all(np.abs(got - want)[seen] <= tol[seen])
+
+
+@pytest.mark.parametrize("heads,group,d,lens,rows", [
+    (2, 4, 64, [5000, 40], [3, 3]), (16, 16, 64, [230, 233], [230, 190]), (1, 20, 128, [300, 9], [4, 2])])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_in_place_on_every_path(kv4, heads, group, d, lens, rows, dtype):
+    """out = q where steps are shared and joined, in the prompts' kernel, and with
+    more columns than a tile; then with a hint far below the lengths."""
+    say(f"in place {heads}x{group}x{d} {lens} {rows} {dtype}")
+    rng = np.random.default_rng(29)
+    s = Stored(kv4, rng, heads, d, 16, lens, rows)
+    s.fill(rng)
+    nh = heads * group
+    q = queries(rng, s, nh, dtype)
+    want, tol = s.expect(q, nh, True, 0, d ** -0.5, dtype)
+    s.batch.reserve(s.cache, nh)
+    tq = torch.from_numpy(q.reshape(s.m, -1)).cuda()
+    s.kv4.kvAttn(tq, tq, s.cache, s.batch, nh)
+    torch.cuda.synchronize()
+    check(tq.cpu().numpy().reshape(q.shape).astype(np.float64), want, tol, dtype, "in place:")
+    b = kv4.Batch(s.batch.table, s.batch.lens, rows=max(rows), row_off=s.batch.row_off, m=s.m, len_max=5)
+    tq = torch.from_numpy(q.reshape(s.m, -1)).cuda()
+    out = torch.empty_like(tq)
+    s.kv4.kvAttn(out, tq, s.cache, b, nh)
+    torch.cuda.synchronize()
+    check(out.cpu().numpy().reshape(q.shape).astype(np.float64), want, tol, dtype, "hint:")
