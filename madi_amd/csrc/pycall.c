@@ -185,7 +185,8 @@ static PyObject *rows(PyObject *mod, PyObject *const *args, Py_ssize_t n) {
            (item(st, 1) == item(shape, 2) || item(shape, 1) == 1);
     if (ok && item(shape, 0) >= m) {
       ld = item(st, 0);
-      if (item(shape, 0) <= 1 && ld < width) ld = width;
+      if (item(shape, 0) <= 1 && (ld < width || ld > UINT32_MAX)) ld = width;
+      if (ld > UINT32_MAX) ld = -1; /* (the library's distances are 32-bit) */
     }
   }
   Py_XDECREF(shape);

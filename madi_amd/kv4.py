@@ -157,6 +157,8 @@ def kvAttn(out, q, cache: KV4, batch: Batch, nh: int, causal: bool = True, windo
     """out = softmax(scale q K^T) V over the cache, scale 1 / sqrt(dim) by
     default.  causal: a row sees the positions up to its own, the last `window`
     of them where window is not 0; else all of its sequence (cross-attention)."""
+    if not 0 <= window < 1 << 32:  # (an argument of 32 bits: others would wrap)
+        raise MadiError(-5, "kvAttn", f"window {window}")
     ldo, ldq, dt = _pair(out, q, batch.m, nh * cache.dim, "kvAttn")
     calls.madi_kv4_attn(out, q, cache.addr, batch.addr, nh, ldo, ldq, window, 1 if causal else 0, dt,
                         cache.scale if scale is None else scale)

@@ -195,3 +195,23 @@ def test_a_call_without_rows():
     b = batch(b=0, m=0)
     assert call("madi_kv4_store", cache(), b, None, None, 128, 128, 0) == -8  # (madi_init, as for any other call)
     assert call("madi_kv4_attn", None, None, cache(), b, 4, 256, 256, 0, 1, 0, 0.125) == -8
+
+
+def test_wrappers_refuse_what_32_bits_do_not_hold():
+    """Distances and windows past 32 bits would wrap to other, valid ones."""
+    c = kv4.KV4(torch.zeros(4 * 2 * R.block_bytes(16, 64), dtype=torch.uint8), page=16, heads=2, dim=64)
+    table, lens = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    b, one = kv4.Batch(table, lens, rows=2), kv4.Batch(table, lens, rows=1)
+    far = torch.empty_strided((2, 128), ((1 << 32) + 128, 1), dtype=torch.float16, device="meta")
+    near = torch.zeros(2, 128, dtype=torch.float16)
+    for f in (lambda: kv4.kvStore(c, b, far, far), lambda: kv4.kvLoad(c, b, near, far),
+              lambda: kv4.kvAttn(far, near, c, b, nh=2), lambda: kv4.kvAttn(near, near, c, b, nh=2, window=(1 << 32) + 5),
+              lambda: kv4.kvAttn(near, near, c, b, nh=2, window=-1)):
+        with pytest.raises(madi_amd.MadiError) as e:
+            f()
+        assert e.value.code == -5
+    # a single row is not apart from any other
+    for k in (torch.empty_strided((1, 128), ((1 << 32) + 128, 1), dtype=torch.float16, device="meta"),):
+        with pytest.raises(madi_amd.MadiError) as e:
+            kv4.kvStore(c, one, k, near[:1])
+        assert e.value.code == -6  # (a meta tensor has no address)
