@@ -46,6 +46,14 @@ inline bool kv4_overlap(const void *a, size_t an, const void *b, size_t bn) {
 __device__ inline uint32_t kv4_const(const uint32_t *p) {
   return *(const __attribute__((address_space(4))) uint32_t *)(uintptr_t)p;
 }
+// Two scales as the most that a store writes, 9352, where they are more, infinite or no
+// numbers, or negative: bits that no store wrote, at positions that a row does not
+// see, times a weight of 0 are 0 then.
+__device__ inline uint32_t kv4_finite(uint32_t w) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  const u16x2 s = __builtin_bit_cast(u16x2, w), most = {0x7091, 0x7091};
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(s, most));
+}
 // One sequence of the batch: its length, its rows [row0, row0 + nrows) of the
 // inputs and outputs, and the position of the first.
 struct Kv4Seq {

@@ -367,9 +367,10 @@ __device__ inline void scores(float (&x)[8], const Query<NB, P> &Q, const Step<N
 }
 
 // A step that some column does not see all of.  First the scales of what lies
-// past the end or stands in for a page that is not there become 0 (those bits may be
-// anything, and 0 times an infinity is not 0), then the scores of the keys that
-// the lane's column does not see, [lo, hi) it does, - infinity.
+// past the end or stands in for a page that is not there become 0, and the others
+// finite (the bits of a key that is not seen may be anything, and 0 times an infinity is
+// not 0), then the scores of the keys that the lane's column does not see, [lo, hi)
+// it does, - infinity.
 template <int NB>
 __device__ inline void cut_scales(Step<NB> &t, int32_t key, int32_t len, uint32_t r, uint32_t g) {
 #pragma unroll
@@ -379,7 +380,7 @@ __device__ inline void cut_scales(Step<NB> &t, int32_t key, int32_t len, uint32_
     uint32_t keep = t.there[i] && k < len ? 0xffffu : 0;
     if (t.there[i] && k + 1 < len) keep |= 0xffff0000u;
 #pragma unroll
-    for (int n = 0; n < Step<NB>::kScaleWords; ++n) t.s[i][n] &= keep;
+    for (int n = 0; n < Step<NB>::kScaleWords; ++n) t.s[i][n] = kv4_finite(t.s[i][n]) & keep;
   }
 }
 template <int NB>
@@ -899,8 +900,9 @@ struct Words {
     const uint32_t b = part + i * kPer;
     return NB % kPer == 0 || b < NB ? b : NB - 1;  // (the last one twice)
   }
-  __device__ inline void fetch(const Kv4Args &a, uint32_t page, uint32_t head, int32_t key, int32_t len, uint32_t part,
-                               uint32_t lane) {
+  // [lo, hi): the keys that every column of the workgroup sees.
+  __device__ inline void fetch(const Kv4Args &a, uint32_t page, uint32_t head, int32_t key, int32_t len, int32_t lo,
+                               int32_t hi, uint32_t part, uint32_t lane) {
     constexpr uint32_t D = NB * 32;
     const uint32_t r = lane & 15, g = lane >> 4;
     there = key < len && page < a.n_pages;
@@ -919,14 +921,15 @@ struct Words {
       s[i][1] = w.y;
     }
     ks = *reinterpret_cast<const uint32_t *>(sp + 4 * (r < 2 * NB ? r : 2 * NB - 1));
-    // V past the end or of a page that is not there: scale 0 (any bits may lie there)
-    if (there && key + 16 <= len) return;
+    // V past the end or of a page that is not there: scale 0; of a key that a column does
+    // not see: a finite one (any bits may lie there)
+    if (there && key >= lo && key + 16 <= hi) return;
     const int32_t at = key + 4 * (int32_t)g;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const uint32_t keep = there && at + 2 * j < len ? (at + 2 * j + 1 < len ? 0xffffffffu : 0xffffu) : 0;
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) s[i][j] &= keep;
+      for (int i = 0; i < kBlocks; ++i) s[i][j] = kv4_finite(s[i][j]) & keep;
     }
   }
   // Its i-th block as operands, for tile `tile` of a buffer.
@@ -989,8 +992,16 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PA
     return kv4_const(a.kv.table + (size_t)t.seq * a.kv.max_pages + (i < a.kv.max_pages ? i : 0));
   };
   uint32_t page = page_of(c);
+  // keys that every column of the workgroup sees
+  int32_t every_lo = 0, every_hi = s.len;
+  if (a.causal) {
+    const uint32_t last = (t.col0 + COLS < t.cols ? t.col0 + COLS : t.cols) - 1;
+    const int32_t p0 = s.pos0 + (int32_t)(t.col0 / a.group), p1 = s.pos0 + (int32_t)(last / a.group);
+    every_hi = p0 + 1 < every_hi ? p0 + 1 : every_hi;
+    if (a.window && p1 >= (int32_t)a.window) every_lo = p1 - (int32_t)a.window + 1;
+  }
   auto fetch = [&](int32_t n) {
-    words.fetch(a.kv, page, head, key_of(n), s.len, part, lane);
+    words.fetch(a.kv, page, head, key_of(n), s.len, every_lo, every_hi, part, lane);
     page = page_of(n + 1);
   };
   auto put = [&](int i, int32_t n) { words.put(i, buf[n & 1], m, fac, my_tile, part, lane); };
