@@ -50,12 +50,20 @@ constexpr int kKeys = 32;  // keys of a step
 constexpr int kPromptWaves = 8;
 constexpr int prompt_tiles(int d, bool f32) { return d < 128 || (d == 128 && !f32) ? 2 : 1; }
 constexpr int prompt_keys(int d) { return d == 256 ? 32 : 64; }
-constexpr float kNever = -1e30f;  // reference before any key was seen
+constexpr float kNever = -__FLT_MAX__;  // reference before any key was seen
 // P is 2^(x - M) with M at first the largest x - 7, raised when an x passes M
 // by 14: P at most 2^14, P s 2^-e at most 2^15 (f16 holds 2^16), and what
 // rounds to nothing is 2^-32 of the largest P at the largest s.  (A reference that
 // follows the largest score at each step would rescale 32 registers each time.)
 constexpr float kLift = 7.0f, kRaise = 14.0f;
+// Scores this far from 0 have f32 neighbours 2^-3 and more away (at 2^28 32, at 10^30 2^76),
+// and M - 7 is no number there.  A column whose largest score is as far takes that
+// score itself as the reference M, without e, and raises it with every larger one: P is at
+// most 1, P s at most 9352.  A score is rounded before its reference is taken off, which
+// is exact then: a multiply-add would leave in what the rounding of the reference
+// took, 2^-24 of 10^10.  (Seven instructions more in 326; the longest caches' times are the same.)
+constexpr float kFar = 0x1p20f;
+__device__ inline bool is_far(float limit) { return !(__builtin_fabsf(limit) < kFar); }
 
 // What a segment costs beside its steps (finding it, its queries, the first
 // words' latency, the waves' results put together), in steps.  (4, 8, 12 and 16 were
@@ -240,8 +248,8 @@ __device__ inline void read_step(Step<NB> &t, const uint8_t *slot, uint32_t ther
 template <int NB>
 struct Acc {
   f32x4 o[2 * NB];     // O^T tiles, scaled like P
-  float ref, sum;      // M + e, and this lane's part of the sum of P 2^-e
-  float limit;         // M + kRaise
+  float ref, sum;      // M + e (far: M), and this lane's part of the sum of P 2^-e
+  float limit;         // M + kRaise (far, or no key seen: M)
   float e, most;       // the column's e, and the largest V scale that it serves
   float check;         // lanes of V scales: the least `most` of all columns; else infinity
 };
@@ -443,14 +451,14 @@ __device__ inline void raise(Acc<NB> &A, const VScales<NB> &c, const float (&x)[
     big = max_across(big);
   }
   top = max_across(top);
-  // the reference of a column that has seen no key stays
-  if (top > A.limit) A.limit = top - kLift + kRaise;
+  if (top > A.limit) A.limit = is_far(top) ? top : top - kLift + kRaise;
   if (big > A.most) {
     const int e = __builtin_amdgcn_frexp_expf(big);
     A.e = (float)e;
     A.most = __builtin_ldexpf(2.0f, e);
   }
-  const float ref = A.limit - kRaise + A.e, f = __builtin_amdgcn_exp2f(A.ref - ref);
+  // (that of a column that has seen no key stays kNever)
+  const float ref = is_far(A.limit) ? A.limit : A.limit - kRaise + A.e, f = __builtin_amdgcn_exp2f(A.ref - ref);
   A.ref = ref;
   A.sum *= f;
   rescale(A, f);
@@ -461,9 +469,11 @@ __device__ inline void raise(Acc<NB> &A, const VScales<NB> &c, const float (&x)[
 // Softmax weights of a step and their product with V.
 template <int NB, int P>
 __device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const Step<NB> &t, const Masks &m, bool whole) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= fac;
   float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3])),
                               __builtin_fmaxf(__builtin_fmaxf(x[4], x[5]), __builtin_fmaxf(x[6], x[7])));
-  top *= fac;
   VScales<NB> c;
   float big = 0;
 #pragma unroll
@@ -478,7 +488,7 @@ __device__ inline void add_values(Acc<NB> &A, float (&x)[8], float fac, const St
   if (__any(top > A.limit || big > A.check)) raise<NB>(A, c, x, top, big, whole);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], fac, -A.ref));
+    x[i] = __builtin_amdgcn_exp2f(x[i] - A.ref);
     A.sum += x[i];
   }
   each<NB>([&](auto B) {
@@ -962,6 +972,7 @@ struct Words {
 
 template <int NB, typename T>
 __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PARAMS, AttnArgs a) {
+#pragma clang fp contract(off)  // (a score is rounded before its reference is taken off, see kFar)
   a.kv = KV4_GATHER;
   constexpr int P = sizeof(T) == 4 ? 2 : 1, NW = kPromptWaves;
   constexpr int D = NB * 32, KC = prompt_keys(D), KT = KC / 16, CT = prompt_tiles(D, sizeof(T) == 4);
@@ -1145,9 +1156,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PA
         if (P == 2) x[ct][n] *= Q[ct].fac;  // 2^-k of the row
         top = __builtin_fmaxf(top, x[ct][n]);
       }
-      if (__any(top > A[ct].ref + kRaise)) {
+      // (their difference is exact where it decides; a sum of large numbers is not)
+      if (__any(top - A[ct].ref > kRaise)) {
         top = max_across(top);
-        const float ref = top > A[ct].ref + kRaise ? top - kLift : A[ct].ref;
+        const float ref = top - A[ct].ref > kRaise ? top - kLift : A[ct].ref;
         const float f = __builtin_amdgcn_exp2f(A[ct].ref - ref);
         A[ct].ref = ref;
         A[ct].sum *= f;

@@ -1,0 +1,133 @@
+"""Attention over the 4-bit cache where scores are large: f32 numbers of 10^8 and
+more lie further apart than the softmax's references are from the largest
+score, and beyond 10^30 (below -10^30) there are scores as well.  Tolerances:
+test_gpu_kv4.py's without the score's error, for the rows where that cannot
+matter: the largest score is ahead of the others by more than twice its bound and 64
+more (e^-64 of the others' |V| is below every other term), or the keys are
+all alike, so that the same roundings give them the same score."""
+import numpy as np
+import pytest
+
+import kv4_ref as R
+from test_gpu_kv4 import NP, Setup, check, kv4, say  # noqa: F401
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+PATHS = [
+    # heads, group, d, page, lens, rows, causal: lengths of one among them
+    (2, 2, 64, 16, [1, 200, 1, 70], [1] * 4, True),              # a workgroup per tile and head
+    (1, 4, 128, 16, [1, 300, 33], [1, 5, 2], True),
+    (2, 4, 96, 64, [1, 3000, 1, 2300], [1, 2, 1, 1], True),      # steps shared by workgroups
+    (1, 2, 256, 16, [2100, 1], [1, 1], True),
+    (16, 16, 64, 16, [230, 233], [230, 233], True),              # the prompts' kernel
+    (16, 16, 128, 16, [230, 233], [230, 233], True),
+]
+
+
+def rows_of_one_key(s, q, nh, causal, scale):
+    """Per row and head whether one key decides alone, by the score's bound."""
+    g, alone = nh // s.heads, np.zeros((s.m, nh), bool)
+    for i, n in enumerate(s.lens):
+        kq, ks = s.held[i][:2]
+        r0, r1 = s.off[i], s.off[i + 1]
+        pos = np.array(R.rows_of(n, r1 - r0))[:, None]
+        for h in range(s.heads):
+            qh = q[r0:r1, h * g:(h + 1) * g].astype(np.float64)
+            k = R.value(kq[:, h], ks[:, h])
+            x = (qh.reshape(-1, s.d) @ k.T).reshape(r1 - r0, g, n) * scale
+            if causal:
+                x = np.where((np.arange(n)[None] <= pos)[:, None], x, -np.inf)
+            x = np.sort(x, -1)
+            bound = R.score_error(qh, ks[:, h], scale)
+            alone[r0:r1, h * g:(h + 1) * g] = (x[..., -1] - x[..., -2] > 2 * bound + 64) if n > 1 else True
+    return alone
+
+
+def one_key_outputs(s, q, nh, causal, dtype):
+    """Exact outputs, and the bound of test_gpu_kv4.py where one key's V is the output and
+    scores have no error: the mean |v| is the output's own."""
+    want, _ = s.expect(q, nh, causal, 0, s.d ** -0.5, dtype)
+    n = np.repeat([max(n, 1) for n in s.lens], np.diff(s.off))[:, None, None]
+    unit = 2.0 ** -10 + 2.0 ** -11 if dtype == "f16" else 3 * 2.0 ** -22 + 2.0 ** -24
+    tol = (unit + 32 * 2.0 ** -23 + (n / 32 + 64) * 2.0 ** -24) * np.abs(want)
+    return want, tol + (2.0 ** -25 if dtype == "f16" else 0) + 1e-25  # (e^-64 of the others)
+
+
+@pytest.mark.parametrize("dtype,top", [("f32", 1e7), ("f32", 3e8), ("f32", 1e10), ("f32", 1e34), ("f16", 300),
+                                       ("f16", 6e4)])
+@pytest.mark.parametrize("heads,group,d,page,lens,rows,causal", PATHS)
+def test_large_scores(kv4, heads, group, d, page, lens, rows, causal, dtype, top):
+    say(f"large scores {heads}x{group}x{d} {lens} {rows} {dtype} {top:g}")
+    rng = np.random.default_rng(sum(lens) + d)
+    s = Setup(kv4, rng, heads, d, page, lens, rows)
+    s.fill(rng, spread=1.0 if dtype == "f32" else 1e4)
+    nh = heads * group
+    q = rng.uniform(-1, 1, (s.m, nh, d))
+    q = (q * top).astype(NP[dtype])
+    want, tol = one_key_outputs(s, q, nh, causal, dtype)
+    alone = rows_of_one_key(s, q, nh, causal, d ** -0.5)
+    assert alone.mean() > 0.5, alone.mean()
+    tq = torch.from_numpy(q.reshape(s.m, -1)).cuda()
+    for reserved in (True, False):
+        if reserved:
+            s.batch.reserve(s.cache, nh)
+        else:
+            s.batch._c.work, s.batch._c.work_bytes = None, 0
+        out = torch.full_like(tq, 77.0)
+        kv4.kvAttn(out, tq, s.cache, s.batch, nh, causal=causal)
+        torch.cuda.synchronize()
+        got = out.cpu().numpy().reshape(s.m, nh, d).astype(np.float64)
+        assert np.all(np.isfinite(got))
+        check(got[alone], want[alone], tol[alone], dtype, f"{alone.mean():.2f} of the rows:")
+        # the others are means of V's rows, whatever the weights
+        for i in range(len(lens)):
+            v = R.value(s.held[i][2], s.held[i][3])
+            lo, hi = (f(0).repeat(group, 0) for f in (v.min, v.max))
+            slack = 2.0 ** -9 * np.maximum(np.abs(lo), np.abs(hi))
+            o = got[s.off[i]:s.off[i + 1]]
+            assert np.all(o >= lo - slack) and np.all(o <= hi + slack)
+
+
+@pytest.mark.parametrize("dtype,top", [("f32", 1.0), ("f32", 3e8), ("f32", 1e10), ("f32", -1e32), ("f16", 6e4),
+                                       ("f16", -6e4)])
+@pytest.mark.parametrize("heads,group,d,page,lens,rows,causal", PATHS)
+def test_keys_that_are_alike(kv4, heads, group, d, page, lens, rows, causal, dtype, top):
+    """Every key the same, so every score: the mean of V, however large the score is,
+    and of either sign."""
+    say(f"alike {heads}x{group}x{d} {lens} {rows} {dtype} {top:g}")
+    rng = np.random.default_rng(sum(lens) + d + 1)
+    s = Setup(kv4, rng, heads, d, page, lens, rows)
+    s.fill(rng)
+    code = rng.integers(1, 8, d)
+    scale = np.full(d // 32, 0.75 if dtype == "f32" else 3000, np.float16)
+    for i, n in enumerate(lens):
+        kq, ks, vq, vs, there = s.held[i]
+        kq[:], ks[:] = code, scale
+        for t in range(n):
+            p, o = s.place(i, t)
+            for h in range(heads):
+                R.put(s.data, page, d, p, h, o, kq[t, h], ks[t, h], vq[t, h], vs[t, h])
+    s.dev.copy_(torch.from_numpy(s.data))
+    nh = heads * group
+    q = (rng.uniform(0.5, 1, (s.m, nh, d)) * top).astype(NP[dtype])
+    # the mean of V with equal weights, and of |V|
+    want, tol = np.zeros((s.m, nh, d)), np.zeros((s.m, nh, d))
+    for i, n in enumerate(lens):
+        v = R.value(s.held[i][2], s.held[i][3])
+        for r, pos in enumerate(R.rows_of(n, rows[i])):
+            if pos < 0:
+                continue
+            k = pos + 1 if causal else n
+            o, a, most = (x.repeat(group, 0) for x in (v[:k].mean(0), np.abs(v[:k]).mean(0), np.abs(v[:k]).sum(0)))
+            unit = 2.0 ** -10 if dtype == "f16" else 3 * 2.0 ** -22
+            last = 2.0 ** -11 if dtype == "f16" else 2.0 ** -24
+            want[s.off[i] + r] = o
+            tol[s.off[i] + r] = ((unit + 32 * 2.0 ** -23 + (n / 32 + 64) * 2.0 ** -24) * a + last * np.abs(o) +
+                                 2.0 ** -32 * most + (2.0 ** -25 if dtype == "f16" else 0))
+    tq = torch.from_numpy(q.reshape(s.m, -1)).cuda()
+    out = torch.full_like(tq, 77.0)
+    s.batch.reserve(s.cache, nh)
+    kv4.kvAttn(out, tq, s.cache, s.batch, nh, causal=causal)
+    torch.cuda.synchronize()
+    check(out.cpu().numpy().reshape(s.m, nh, d).astype(np.float64), want, tol, dtype)
