@@ -421,7 +421,8 @@ int madi_kv4_load(void *k, void *v, uint32_t ldk, uint32_t ldv, int dtype, const
  * V scale (single tokens and short prompts) or by itself (long prompts);
  * K and V enter exactly (long prompts: V below 2^-14 to 2^-25).  With f32
  * rows every operand is kept to 22 bits or more of the largest that its row
- * sees; q may be of any magnitude.  out may be q
+ * sees.  q and scale may be of any magnitude, finite, with which f32 holds the scores; a row
+ * with one that it does not is NaN.  out may be q
  * itself (same rows), else it must not overlap it. */
 int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, const madi_kv4_batch *batch,
                   uint32_t nh, uint32_t ldo, uint32_t ldq, uint32_t window, int causal, int dtype,

@@ -272,6 +272,13 @@ struct RawQuery {
     for (int b = 0; b < NB; ++b) x[b] = *reinterpret_cast<const vec8 __attribute__((aligned(16))) *>(q + 32 * b);
   }
 };
+// A scale as the scores' factor.  Never 0, so that it leaves the - infinity of a key not
+// seen what it is, and never infinite, also times a K scale or 2^9, so that a sum of 0 stays
+// 0: sums are multiples of 2^-57, so with 2^100 as with any larger factor the largest
+// decides alone.
+__device__ inline float factor(float scale) {
+  return __builtin_fminf(__builtin_fmaxf(scale * 1.4426950408889634f, 1e-37f), 0x1p100f);
+}
 // As operands.  An f32 row is brought to [2^10, 2^11) by a power of two 2^k, so
 // that its low parts lose nothing that counts.
 template <int NB, int P, typename T>
@@ -286,8 +293,7 @@ __device__ inline void make_query(Query<NB, P> &Q, const RawQuery<NB, T> &raw, b
     top = max_across(top);
     k = top > 0 && top < __builtin_inff() ? 11 - __builtin_amdgcn_frexp_expf(top) : 0;
   }
-  // (never 0, so that it leaves the - infinity of a key not seen what it is)
-  Q.fac = __builtin_fmaxf(__builtin_ldexpf(__builtin_fabsf(scale) * 1.4426950408889634f, -k), 1e-37f);
+  Q.fac = factor(__builtin_ldexpf(__builtin_fabsf(scale), -k));
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     if constexpr (P == 1) {
@@ -990,7 +996,9 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PA
   const uint32_t r = lane & 15, g = lane >> 4;
   const uint32_t my_tile = wave / Wd::kPer, part = wave % Wd::kPer;
   const Masks m = masks();
-  const float fac = __builtin_fmaxf(__builtin_fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
+  // (f32 rows: theirs comes with the row's power of two, of which K scales times one
+  // for all rows would be too large or too small)
+  const float fac = P == 2 ? 1.0f : factor(__builtin_fabsf(a.scale));
 
   const int32_t c_end = ((t.first + t.steps) * kKeys + KC - 1) / KC;
   int32_t c = t.first * kKeys / KC;
@@ -1045,7 +1053,6 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PA
     const RawQuery<NB, T> raw(static_cast<const T *>(a.q) + (size_t)(s.row0 + row) * a.ldq +
                               (size_t)(head * a.group + sub) * D + 8 * g);
     make_query<NB, P, T>(Q[ct], raw, mine[ct], a.scale);
-    Q[ct].fac *= 1 / fac;
     A[ct].ref = kNever;
     A[ct].sum = 0;
 #pragma unroll
@@ -1153,7 +1160,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(KV4_PA
       float top = -__builtin_inff();
 #pragma unroll
       for (int n = 0; n < 4 * KT; ++n) {
-        if (P == 2) x[ct][n] *= Q[ct].fac;  // 2^-k of the row
+        if (P == 2) x[ct][n] *= Q[ct].fac;
         top = __builtin_fmaxf(top, x[ct][n]);
       }
       // (their difference is exact where it decides; a sum of large numbers is not)

@@ -44,10 +44,10 @@ def rows_of_one_key(s, q, nh, causal, scale):
     return alone
 
 
-def one_key_outputs(s, q, nh, causal, dtype):
+def one_key_outputs(s, q, nh, causal, dtype, scale=None):
     """Exact outputs, and the bound of test_gpu_kv4.py where one key's V is the output and
     scores have no error: the mean |v| is the output's own."""
-    want, _ = s.expect(q, nh, causal, 0, s.d ** -0.5, dtype)
+    want, _ = s.expect(q, nh, causal, 0, scale or s.d ** -0.5, dtype)
     n = np.repeat([max(n, 1) for n in s.lens], np.diff(s.off))[:, None, None]
     unit = 2.0 ** -10 + 2.0 ** -11 if dtype == "f16" else 3 * 2.0 ** -22 + 2.0 ** -24
     tol = (unit + 32 * 2.0 ** -23 + (n / 32 + 64) * 2.0 ** -24) * np.abs(want)
@@ -131,3 +131,64 @@ def test_keys_that_are_alike(kv4, heads, group, d, page, lens, rows, causal, dty
     kv4.kvAttn(out, tq, s.cache, s.batch, nh, causal=causal)
     torch.cuda.synchronize()
     check(out.cpu().numpy().reshape(s.m, nh, d).astype(np.float64), want, tol, dtype)
+
+
+@pytest.mark.parametrize("top,scale", [(3e38, 2e-38), (1e36, 1e-36), (1e-36, 1e36)])
+@pytest.mark.parametrize("heads,group,d,page,lens,rows", [(16, 16, 64, 16, [230, 233], [230, 233]),
+                                                           (16, 16, 256, 16, [200, 217], [200, 217])])
+def test_prompts_of_large_and_small_rows(kv4, heads, group, d, page, lens, rows, top, scale):
+    """f32 rows up to the largest numbers and of the smallest, the scale bringing the scores back."""
+    say(f"prompt rows of {top:g}, scale {scale:g}, d {d}")
+    rng = np.random.default_rng(31)
+    s = Setup(kv4, rng, heads, d, page, lens, rows)
+    s.fill(rng, spread=0.01)
+    nh = heads * group
+    q = (rng.uniform(-1, 1, (s.m, nh, d)) * top).astype(np.float32)
+    want, tol = s.expect(q, nh, True, 0, float(np.float32(scale)), "f32")
+    tq = torch.from_numpy(q.reshape(s.m, -1)).cuda()
+    out = torch.full_like(tq, 77.0)
+    kv4.kvAttn(out, tq, s.cache, s.batch, nh, scale=scale)
+    torch.cuda.synchronize()
+    check(out.cpu().numpy().reshape(s.m, nh, d).astype(np.float64), want, tol, "f32")
+
+
+@pytest.mark.parametrize("heads,group,d,page,lens,rows,causal", PATHS)
+def test_rows_of_zeros_under_a_large_scale(kv4, heads, group, d, page, lens, rows, causal):
+    """Rows of 10^-36 with a scale of 10^36, among them (padding) rows of zeros: the mean of V."""
+    say(f"rows of zeros {heads}x{group}x{d} {lens}")
+    rng = np.random.default_rng(sum(lens) + 5)
+    s = Setup(kv4, rng, heads, d, page, lens, rows)
+    s.fill(rng, spread=0.01)
+    nh = heads * group
+    q = (rng.uniform(-1, 1, (s.m, nh, d)) * 1e-36).astype(np.float32)
+    q[rng.random((s.m, nh)) < 0.5] = 0
+    want, tol = s.expect(q, nh, causal, 0, float(np.float32(1e36)), "f32")
+    tq = torch.from_numpy(q.reshape(s.m, -1)).cuda()
+    out = torch.full_like(tq, 77.0)
+    s.batch.reserve(s.cache, nh)
+    kv4.kvAttn(out, tq, s.cache, s.batch, nh, causal=causal, scale=1e36)
+    torch.cuda.synchronize()
+    check(out.cpu().numpy().reshape(s.m, nh, d).astype(np.float64), want, tol, "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,group,d,page,lens,rows,causal", PATHS)
+def test_the_largest_scales(kv4, heads, group, d, page, lens, rows, causal, dtype):
+    """A scale near the end of f32 with small q and K: the largest score decides."""
+    say(f"largest scales {heads}x{group}x{d} {lens} {dtype}")
+    rng = np.random.default_rng(sum(lens) + 6)
+    s = Setup(kv4, rng, heads, d, page, lens, rows)
+    s.fill(rng, spread=1e-5)
+    nh, scale = heads * group, float(np.float32(3e38))
+    q = (rng.uniform(-1, 1, (s.m, nh, d)) * 2.0 ** -10).astype(NP[dtype])
+    alone = rows_of_one_key(s, q, nh, causal, scale)
+    assert alone.mean() > 0.5
+    want, tol = one_key_outputs(s, q, nh, causal, dtype, scale)
+    tq = torch.from_numpy(q.reshape(s.m, -1)).cuda()
+    out = torch.full_like(tq, 77.0)
+    s.batch.reserve(s.cache, nh)
+    kv4.kvAttn(out, tq, s.cache, s.batch, nh, causal=causal, scale=scale)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(s.m, nh, d).astype(np.float64)
+    assert np.all(np.isfinite(got))
+    check(got[alone], want[alone], tol[alone], dtype)
