@@ -98,6 +98,7 @@ class Batch:
             if not 0 <= v < 1 << 31:
                 raise MadiError(-5, "kv4.Batch", f"{what} = {v}")
         self.table, self.lens, self.row_off, self.work = table, lens, row_off, None
+        self._outgrown: list = []
         self.b, self.rows, self.m = b, rows, m
         self._c = _Batch(ptr(table), ptr(lens), ptr(row_off), b, max_pages, rows, m, len_max, None, 0)
         self.addr = ctypes.addressof(self._c)
@@ -105,10 +106,13 @@ class Batch:
     def reserve(self, cache: KV4, nh: int) -> int:
         """Allocate the workspace with which kvAttn splits long caches over
         workgroups as it sees fit; returns its bytes.  (The largest of several
-        caches' or heads' needs is kept.)"""
+        caches' or heads' needs is kept.  A smaller one that was there before lives as
+        long as the Batch: calls still running and captured graphs point to it.)"""
         import torch
         need = int(lib().madi_kv4_attn_bytes(cache.addr, self.addr, nh))
         if need > self._c.work_bytes:
+            if self.work is not None:
+                self._outgrown.append(self.work)
             self.work = torch.empty(need, dtype=torch.uint8, device=self.table.device)
             self._c.work, self._c.work_bytes = self.work.data_ptr(), need
         return need
