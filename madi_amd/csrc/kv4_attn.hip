@@ -1251,7 +1251,10 @@ struct Plan {
 // A cache of up to four steps per wave (2048 keys at d 64) stays with one workgroup
 // per tile and head: eight sequences of 1500, 20 heads of 64, f32, take 13.1 us
 // there and 16.7 dealt out and joined; from more steps per wave on the join is the
-// smaller part.  Longer ones are dealt out over as many workgroups as are
+// smaller part.  Where that is eight waves, though (d 256, f32 rows of d 128), and half of the
+// CUs have a workgroup each, they stay alone up to 64 steps: f32 rows, 8 heads of
+// 128, 1500 keys, 16 sequences 16.0 us alone and 21.4 dealt out, 4 sequences 16.1 and 13.9; of
+// 256 27.1 and 29.6, 26.7 and 19.2.  Longer ones are dealt out over as many workgroups as are
 // resident at once.  most: without the prompts' kernel, whose place
 // depends on the type and window.
 Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype, uint32_t window, uint32_t cus,
@@ -1280,8 +1283,9 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
   p.part = (size_t)kCols * (c->d + 2) * 4;
   const uint64_t items = (uint64_t)p.tiles * b->b;
   p.starts = (size_t)(items + 1) * 4;
-  p.few = (len + kKeys - 1) / kKeys <= kFew;
-  if ((len + kKeys - 1) / kKeys <= 4 * waves_alone(c->d, dtype == MADI_F32)) return p;
+  p.few = steps <= kFew;
+  if (steps <= 4 * waves_alone(c->d, dtype == MADI_F32)) return p;
+  if (steps <= 64 && items * c->nkv >= cus / 2) return p;
   // (the row's places are counted in 32 bits)
   if (items * c->nkv * ((reach + kKeys - 1) / kKeys + kOverhead + 1) > 0x40000000u) return p;
   if (items > 0xfffffu) return p;  // (the join's threads, 4096 per item, likewise)
@@ -1322,9 +1326,12 @@ void launch(const AttnArgs &a, const Plan &p, uint32_t cus) {
 extern "C" size_t madi_kv4_attn_bytes(const madi_kv4 *cache, const madi_kv4_batch *batch, uint32_t nh) {
   Kv4Args a;
   if (kv4_args("madi_kv4_attn_bytes", cache, batch, &a) || nh == 0 || nh % cache->nkv) return 0;
-  // the most that any type and window may take
-  const Plan p = plan_of(cache, batch, nh, MADI_F16, 0, initialized() ? (uint32_t)cu_count() : 256, true);
-  return p.bytes();
+  // the most that any type and window may take (f16 rows have more workgroups, f32 rows of
+  // d 128 are split from shorter caches on)
+  const uint32_t cus = initialized() ? (uint32_t)cu_count() : 256;
+  const size_t h = plan_of(cache, batch, nh, MADI_F16, 0, cus, true).bytes();
+  const size_t f = plan_of(cache, batch, nh, MADI_F32, 0, cus, true).bytes();
+  return h > f ? h : f;
 }
 
 extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, const madi_kv4_batch *batch,

@@ -215,3 +215,15 @@ def test_wrappers_refuse_what_32_bits_do_not_hold():
         with pytest.raises(madi_amd.MadiError) as e:
             kv4.kvStore(c, one, k, near[:1])
         assert e.value.code == -6  # (a meta tensor has no address)
+
+
+@pytest.mark.parametrize("d,whole", [(64, 2048), (96, 2048), (128, 1024), (256, 1024)])
+def test_the_workspace_serves_both_types_at_every_length(d, whole):
+    """Rows of one type are split from shorter caches on than the other's (d = 128: f32
+    from 1025 keys, f16 from 2049): there is a workspace wherever either is."""
+    f = lambda n: call("madi_kv4_attn_bytes", cache(nkv=8, d=d), batch(b=1, max_pages=8192, rows=1, m=1, len_max=n), 32)
+    assert f(whole) == 0
+    for n in (whole + 1, 1500, 2048, 2049, 4096, 131072):
+        assert (f(n) > 0) == (n > whole), n
+    sizes = [f(n) for n in (2049, 4096, 131072)]
+    assert min(sizes) == max(sizes)
