@@ -39,6 +39,12 @@ inline bool kv4_overlap(const void *a, size_t an, const void *b, size_t bn) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return an && bn && x < y + bn && y < x + an;
 }
+// Whether [a, a + an) has a part of the batch's table, lens or row_off, which kernels take
+// for constant while they write there.
+inline bool kv4_on_batch(const madi_kv4_batch *b, const void *a, size_t an) {
+  return kv4_overlap(a, an, b->table, (size_t)b->b * b->max_pages * 4) || kv4_overlap(a, an, b->lens, (size_t)b->b * 4) ||
+         (b->row_off && kv4_overlap(a, an, b->row_off, ((size_t)b->b + 1) * 4));
+}
 
 // ---------------------------------------------------------------- device side
 // A number that no kernel writes while others read it: at a uniform address one

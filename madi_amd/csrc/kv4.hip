@@ -317,6 +317,8 @@ int run(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, void *k, v
   const size_t cb = kv4_cache_bytes(c);
   if (kv4_overlap(k, kb, c->data, cb) || kv4_overlap(v, vb, c->data, cb))
     return fail(MADI_ERR_ARG, "%s: k or v lies in the cache", what);
+  if (STORE ? kv4_on_batch(b, c->data, cb) : kv4_on_batch(b, k, kb) || kv4_on_batch(b, v, vb))
+    return fail(MADI_ERR_ARG, "%s: %s on table, lens or row_off", what, STORE ? "the cache lies" : "k or v lie");
   // K and V rows may alternate in one buffer; the extents overlap then, the rows do not
   if (!STORE && kv4_overlap(k, kb, v, vb)) {
     const size_t es = dtype == MADI_F32 ? 4 : 2, row = (size_t)ldk * es, w = (size_t)width * es;

@@ -1356,6 +1356,8 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
       kv4_overlap(out, ob, batch->work, wb) || kv4_overlap(q, qb, batch->work, wb) ||
       kv4_overlap(cache->data, cb, batch->work, wb))
     return fail(MADI_ERR_ARG, "%s: out or work overlaps another operand", what);
+  if (kv4_on_batch(batch, out, ob) || kv4_on_batch(batch, batch->work, wb))
+    return fail(MADI_ERR_ARG, "%s: out or work overlaps table, lens or row_off", what);
   if ((uint64_t)batch->rows * (nh / cache->nkv) > 0x7fffffffu)
     return fail(MADI_ERR_SHAPE, "%s: %u rows of a sequence in one call", what, batch->rows);
   if (!initialized()) return fail(MADI_ERR_NOT_INIT, "%s: madi_init has not succeeded", what);

@@ -227,3 +227,28 @@ def test_the_workspace_serves_both_types_at_every_length(d, whole):
         assert (f(n) > 0) == (n > whole), n
     sizes = [f(n) for n in (2049, 4096, 131072)]
     assert min(sizes) == max(sizes)
+
+
+@pytest.mark.parametrize("what,size", [("table", 16), ("lens", 8), ("row_off", 12)])
+def test_what_a_call_reads_is_not_written_by_it(what, size):
+    """table, lens and row_off under out, work, k, v or the cache are refused, beside
+    them taken; under what a call only reads too."""
+    c, x, y = cache(), FAR + 0x100000, FAR + 0x200000
+    work = dict(work=FAR + 0x900000, work_bytes=512)
+    rows, attn, held = (5 * 256 + 128) * 2, 6 * 256 * 2, 4 * 2 * R.block_bytes(16, 64)
+    writes = [
+        (x, rows, lambda b: call("madi_kv4_load", x, y, 256, 256, 0, c, b)),
+        (y, rows, lambda b: call("madi_kv4_load", x, y, 256, 256, 0, c, b)),
+        (x, attn, lambda b: call("madi_kv4_attn", x, y, c, b, 4, 256, 256, 0, 1, 0, 0.125)),
+        (work["work"], 512, lambda b: call("madi_kv4_attn", x, y, c, b, 4, 256, 256, 0, 1, 0, 0.125)),
+        (FAKE, held, lambda b: call("madi_kv4_store", c, b, x, y, 256, 256, 0)),
+    ]
+    for start, length, f in writes:
+        for at, code in ((start - size, -8), (start - size + 4, -9), (start, -9), (start + length - 4, -9),
+                         (start + length, -8)):
+            assert f(batch(**{"row_off": FAR, **work, what: at})) == code, (hex(at), _lib.last_error())
+    for at in (x, y):
+        assert call("madi_kv4_store", c, batch(**{"row_off": FAR, what: at}), x, y, 256, 256, 0) == -8
+    assert call("madi_kv4_attn", x, y, c, batch(**{"row_off": FAR, what: y}), 4, 256, 256, 0, 1, 0, 0.125) == -8
+    # (of one token: no row starts are read without row_off)
+    assert call("madi_kv4_attn", x, y, c, batch(), 4, 256, 256, 0, 1, 0, 0.125) == -8
