@@ -30,7 +30,7 @@ typedef struct {
   PyObject *name, *fail;
 } Call;
 
-static PyObject *s_data_ptr, *s_dtype, *s_shape, *s_stride;
+static PyObject *s_data_ptr, *s_dtype, *s_shape, *s_stride, *s_get_device;
 
 /* An integer's value modulo 2^64, as ctypes takes it (anything with
  * __index__; the callee of a 32-bit argument reads the low half). */
@@ -157,18 +157,27 @@ static PyObject *bind(PyObject *mod, PyObject *args) {
   return (PyObject *)c;
 }
 
-/* rows(t, m, width, f16, f32) -> 2 * ld + code: a tensor's rows as a pointer and
+/* rows(t, m, width, f16, f32, device) -> 2 * ld + code: a tensor's rows as a pointer and
  * a distance.  t is [rows][width] or [rows][a][b], a * b = width, at least m
  * rows, of dtype f16 (code 0) or f32 (code 1), the elements of a row contiguous; ld is
  * the distance of its rows in elements (of a single row at least width).
- * -1 for any other tensor.  (0.8 us in Python, 0.3 here; a call has two to check.) */
+ * -1 for any other tensor, -2 for one that is not on GPU `device` (below 0: not looked
+ * at).  (0.8 us in Python, 0.3 here; a call has two to check.) */
 static long long item(PyObject *tuple, Py_ssize_t i) { return PyLong_AsLongLong(PyTuple_GET_ITEM(tuple, i)); }
 
 static PyObject *rows(PyObject *mod, PyObject *const *args, Py_ssize_t n) {
   (void)mod;
-  if (n != 5) return PyErr_Format(PyExc_TypeError, "rows takes 5 arguments (%zd given)", n);
-  const long long m = PyLong_AsLongLong(args[1]), width = PyLong_AsLongLong(args[2]);
+  if (n != 6) return PyErr_Format(PyExc_TypeError, "rows takes 6 arguments (%zd given)", n);
+  const long long m = PyLong_AsLongLong(args[1]), width = PyLong_AsLongLong(args[2]), device = PyLong_AsLongLong(args[5]);
   if (PyErr_Occurred()) return NULL;
+  if (device >= 0) {
+    PyObject *on = PyObject_CallMethodNoArgs(args[0], s_get_device);
+    if (!on) return NULL;
+    const int there = PyLong_AsLongLong(on) == device;
+    Py_DECREF(on);
+    if (PyErr_Occurred()) return NULL;
+    if (!there) return PyLong_FromLong(-2);
+  }
   PyObject *dtype = PyObject_GetAttr(args[0], s_dtype);
   if (!dtype) return NULL;
   const int code = dtype == args[3] ? 0 : dtype == args[4] ? 1 : -1;
@@ -196,7 +205,7 @@ static PyObject *rows(PyObject *mod, PyObject *const *args, Py_ssize_t n) {
 }
 
 static PyMethodDef methods[] = {{"rows", (PyCFunction)(void (*)(void))rows, METH_FASTCALL,
-                                 "rows(t, m, width, f16, f32) -> 2 * ld + code, or -1"},
+                                 "rows(t, m, width, f16, f32, device) -> 2 * ld + code, -1 or -2"},
                                 {"bind", bind, METH_VARARGS, "bind(address, signature, name, fail)"},
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", NULL, -1, methods, NULL, NULL, NULL, NULL};
@@ -207,5 +216,6 @@ PyMODINIT_FUNC PyInit__pycall(void) {
   s_dtype = PyUnicode_InternFromString("dtype");
   s_shape = PyUnicode_InternFromString("shape");
   s_stride = PyUnicode_InternFromString("stride");
-  return s_data_ptr && s_dtype && s_shape && s_stride ? PyModule_Create(&module) : NULL;
+  s_get_device = PyUnicode_InternFromString("get_device");
+  return s_data_ptr && s_dtype && s_shape && s_stride && s_get_device ? PyModule_Create(&module) : NULL;
 }

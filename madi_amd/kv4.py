@@ -12,7 +12,8 @@ each argument may be).
 Rows are torch tensors of float16 or float32, [m][heads * dim] or [m][heads][dim]
 with the elements of a row contiguous (a slice of a stacked projection's output is fine).
 Work is enqueued on the library's stream (madi_amd.q8.init).  As in madi_amd.q8,
-a refused call raises MadiError.
+a refused call raises MadiError; tensors in host memory or on another GPU than the
+library's are refused.
 """
 from __future__ import annotations
 
@@ -45,6 +46,29 @@ def _bytes(n_pages: int, page: int, heads: int, dim: int) -> int:
     return n
 
 
+DEVICE = 0  # the library's (madi_init)
+
+
+def _on(what, *tensors) -> int:
+    """0 where all are on the library's device, else another number."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise MadiError(-9, what, f"tensors on {' and '.join(sorted(map(str, devices)))}")
+    device = devices.pop()
+    return 0 if device.type == "cuda" and device.index == DEVICE else -1
+
+
+def _device(cache, batch, what: str) -> int:
+    """The device that a call's rows have to be on.  (Without one the library refuses
+    every call by itself: -1, any will do.)"""
+    if cache.on | batch.on:
+        if lib().madi_device_cu_count():
+            raise MadiError(-9, what, f"cache and batch must be in the memory of GPU {DEVICE}, "
+                                      f"are on {cache.data.device} and {batch.table.device}")
+        return -1
+    return DEVICE
+
+
 class KV4:
     """A pool of pages over `data`, a contiguous device tensor of at least
     madi_kv4_bytes bytes (one pool per layer)."""
@@ -57,6 +81,7 @@ class KV4:
             raise MadiError(-5, "kv4.KV4", f"data must be contiguous and hold {n_pages} pages, has {held} bytes")
         self.data, self.page, self.heads, self.dim, self.n_pages = data, page, heads, dim, n_pages
         self.width, self.scale = heads * dim, 1.0 / math.sqrt(dim)
+        self.on = _on("kv4.KV4", data)
         self._c = _Cache(data.data_ptr(), n_pages, page, heads, dim)
         self.addr = ctypes.addressof(self._c)
 
@@ -100,6 +125,7 @@ class Batch:
         self.table, self.lens, self.row_off, self.work = table, lens, row_off, None
         self._outgrown: list = []
         self.b, self.rows, self.m = b, rows, m
+        self.on = _on("kv4.Batch", table, lens, row_off)
         self._c = _Batch(ptr(table), ptr(lens), ptr(row_off), b, max_pages, rows, m, len_max, None, 0)
         self.addr = ctypes.addressof(self._c)
 
@@ -121,7 +147,7 @@ class Batch:
 _check: tuple = ()
 
 
-def _rows(t, m: int, width: int, what: str) -> int:
+def _rows(t, m: int, width: int, device: int, what: str) -> int:
     """2 * row distance + dtype code of rows [m][width].  (Rows that are not apart, a
     broadcast's, are left to the library to refuse.)"""
     global _check
@@ -130,15 +156,18 @@ def _rows(t, m: int, width: int, what: str) -> int:
         from ._pycall import rows
         _check = rows, torch.float16, torch.float32
     rows, f16, f32 = _check
-    r = rows(t, m, width, f16, f32)
+    r = rows(t, m, width, f16, f32, device)
+    if r == -2:
+        raise MadiError(-9, what, f"rows must be in the memory of GPU {device}, are on {t.device}")
     if r < 0:
         raise MadiError(-5, what, f"rows must be float16 or float32 [{m}][{width}] with contiguous rows; "
                                   f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
     return r
 
 
-def _pair(a, b, m: int, width: int, what: str):
-    a, b = _rows(a, m, width, what), _rows(b, m, width, what)
+def _pair(a, b, cache: KV4, batch: Batch, width: int, what: str):
+    device = _device(cache, batch, what)
+    a, b = _rows(a, batch.m, width, device, what), _rows(b, batch.m, width, device, what)
     if (a ^ b) & 1:
         raise MadiError(-9, what, "the two tensors are of two types")
     return a >> 1, b >> 1, a & 1
@@ -146,13 +175,13 @@ def _pair(a, b, m: int, width: int, what: str):
 
 def kvStore(cache: KV4, batch: Batch, k, v) -> None:
     """Quantise rows k, v into the cache, at each sequence's last positions."""
-    ldk, ldv, dt = _pair(k, v, batch.m, cache.width, "kvStore")
+    ldk, ldv, dt = _pair(k, v, cache, batch, cache.width, "kvStore")
     calls.madi_kv4_store(cache.addr, batch.addr, k, v, ldk, ldv, dt)
 
 
 def kvLoad(cache: KV4, batch: Batch, k, v) -> None:
     """Read each sequence's last rows back into k, v."""
-    ldk, ldv, dt = _pair(k, v, batch.m, cache.width, "kvLoad")
+    ldk, ldv, dt = _pair(k, v, cache, batch, cache.width, "kvLoad")
     calls.madi_kv4_load(k, v, ldk, ldv, dt, cache.addr, batch.addr)
 
 
@@ -163,7 +192,7 @@ def kvAttn(out, q, cache: KV4, batch: Batch, nh: int, causal: bool = True, windo
     of them where window is not 0; else all of its sequence (cross-attention)."""
     if not 0 <= window < 1 << 32:  # (an argument of 32 bits: others would wrap)
         raise MadiError(-5, "kvAttn", f"window {window}")
-    ldo, ldq, dt = _pair(out, q, batch.m, nh * cache.dim, "kvAttn")
+    ldo, ldq, dt = _pair(out, q, cache, batch, nh * cache.dim, "kvAttn")
     calls.madi_kv4_attn(out, q, cache.addr, batch.addr, nh, ldo, ldq, window, 1 if causal else 0, dt,
                         cache.scale if scale is None else scale)
 
