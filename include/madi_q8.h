@@ -361,8 +361,8 @@ int madi_flash_enc_f16(void *out, const void *q, const void *k, const void *v, u
  *   scales page * d/8 bytes: tokens 4u..4u+3 at u * d/2; f16 (x, b, t) at
  *          ((x * nb + b) * 4 + t) * 2, x = 0 for K and 1 for V, t the token - 4u
  * d is 64, 96, 128 or 256; page a power of two from 16 to 2^20; data 16-byte
- * aligned, 2^48 bytes at most.  madi_kv4_bytes gives the size of data (0 for a
- * shape it does not take). */
+ * aligned, 2^48 bytes at most; a table reaches 2^31 - 4096 positions at most.
+ * madi_kv4_bytes gives the size of data (0 for a shape it does not take). */
 typedef struct {
   void *data;       /* device */
   uint32_t n_pages; /* pages in the pool */

@@ -44,8 +44,9 @@ int kv4_args(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, Kv4Ar
   if (!b->row_off && (uint64_t)b->b * b->rows != b->m)
     return fail(MADI_ERR_SHAPE, "%s: m = %u is not b * rows = %u * %u", what, b->m, b->b, b->rows);
   if (b->b && b->max_pages == 0) return fail(MADI_ERR_SHAPE, "%s: max_pages is 0", what);
-  if ((uint64_t)b->max_pages * c->page > 0x7fffffffu)
-    return fail(MADI_ERR_SHAPE, "%s: max_pages * page = %u * %u positions (below 2^31)", what,
+  // (positions are int32_t, and a kernel's steps and chunks end a little past the last one)
+  if ((uint64_t)b->max_pages * c->page > 0x7ffff000u)
+    return fail(MADI_ERR_SHAPE, "%s: max_pages * page = %u * %u positions (at most 2^31 - 4096)", what,
                 b->max_pages, c->page);
   if (!c->data || (b->b && (!b->table || !b->lens)))
     return fail(MADI_ERR_NULL, "%s: null pointer", what);
@@ -159,8 +160,8 @@ __device__ inline bool unit_of(const Kv4Args &a, uint32_t per_quad, Unit &u) {
   const uint32_t l = threadIdx.x & 15, hb = part * 16 + (threadIdx.x >> 4);
   u.seq = blockIdx.y;
   u.s = kv4_seq(a, u.seq);
+  if (quad * 4 >= ((uint32_t)u.s.pos0 & 3) + u.s.nrows || hb >= a.nkv * NB) return false;
   u.first = ((u.s.pos0 >> 2) + (int32_t)quad) * 4;
-  if (u.first >= u.s.pos0 + (int32_t)u.s.nrows || hb >= a.nkv * NB) return false;
   u.h = hb / NB;
   u.b = hb % NB;
   u.tok = l & 3;

@@ -252,3 +252,16 @@ def test_what_a_call_reads_is_not_written_by_it(what, size):
     assert call("madi_kv4_attn", x, y, c, batch(**{"row_off": FAR, what: y}), 4, 256, 256, 0, 1, 0, 0.125) == -8
     # (of one token: no row starts are read without row_off)
     assert call("madi_kv4_attn", x, y, c, batch(), 4, 256, 256, 0, 1, 0, 0.125) == -8
+
+
+def test_positions_end_before_31_bits_do():
+    """A step of keys that begins below 2^31 would end past it: the last 4096 positions
+    are refused."""
+    k, v = FAR + 0x100000, FAR + 0x200000
+    for page, most in ((16, (1 << 31) - 4096), (4096, (1 << 31) - 4096), (1 << 20, (1 << 31) - (1 << 20))):
+        c = cache(page=page)
+        for pages, code in ((most // page, -8), (most // page + 1, -5)):
+            b = batch(max_pages=pages, table=FAR + (1 << 32))
+            assert call("madi_kv4_store", c, b, k, v, 128, 128, 0) == code
+            assert call("madi_kv4_load", k, v, 128, 128, 0, c, b) == code
+            assert call("madi_kv4_attn", k, v, c, b, 4, 256, 256, 0, 1, 0, 0.125) == code
