@@ -135,6 +135,8 @@ class Batch:
         caches' or heads' needs is kept.  A smaller one that was there before lives as
         long as the Batch: calls still running and captured graphs point to it.)"""
         import torch
+        if not 1 <= nh < 1 << 32 or nh % cache.heads:  # (the library would ask for no bytes)
+            raise MadiError(-5, "kv4.Batch.reserve", f"{nh} query heads over {cache.heads} kv heads")
         need = int(lib().madi_kv4_attn_bytes(cache.addr, self.addr, nh))
         if need > self._c.work_bytes:
             if self.work is not None:

@@ -83,3 +83,12 @@ def test_indices_on_two_devices_are_refused():
         assert e.value.code == -9
     with pytest.raises(madi_amd.MadiError):
         kv4.Batch(table, lens, row_off=torch.zeros(3, dtype=torch.int32, device="meta"), m=2)
+
+
+def test_reserve_refuses_head_counts_that_attention_refuses():
+    batch = kv4.Batch(*indices(), rows=1)
+    for nh in (0, 3, -2, 1, (1 << 32) + 2):
+        with pytest.raises(madi_amd.MadiError) as e:
+            batch.reserve(pool(), nh=nh)
+        assert e.value.code == -5
+    assert batch.work is None and batch.reserve(pool(), nh=6) > 0
