@@ -419,11 +419,12 @@ int madi_kv4_load(void *k, void *v, uint32_t ldk, uint32_t ldv, int dtype, const
  * see leaves no trace in it, whatever it holds.  Scores, softmax and sums are
  * f32.  With f16 rows a probability enters the product as one f16, times its
  * V scale (single tokens and short prompts) or by itself (long prompts);
- * K and V enter exactly (long prompts: V below 2^-14 to 2^-25).  With f32
- * rows every operand is kept to 22 bits or more of the largest that its row
- * sees.  q and scale may be of any magnitude, finite, with which f32 holds the scores; a row
- * with one that it does not is NaN.  out may be q
- * itself (same rows), else it must not overlap it. */
+ * K and V enter exactly.  With f32 rows every operand is kept to 22 bits or
+ * more of the largest that its row sees.  (Long prompts hold V as two f16; where V is
+ * below 2^-14 the matrix core adds up its products to 2^-18 of their magnitudes.)  q and
+ * scale may be of any magnitude, finite, with which f32 holds the scores; a row with
+ * one that it does not is NaN.  out may be q itself (same rows), else it must
+ * not overlap it. */
 int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, const madi_kv4_batch *batch,
                   uint32_t nh, uint32_t ldo, uint32_t ldq, uint32_t window, int causal, int dtype,
                   float scale);

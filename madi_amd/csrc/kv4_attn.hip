@@ -888,7 +888,10 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(KV4_PARAMS, AttnArgs 
 // registers.  The operands lie in LDS as the MFMAs read them, 16 bytes per lane.
 //   K as its codes (the block sums get their scales, f32 in LDS, afterwards);
 //   V as (n - 8) s in two f16, which hold all of its 15 bits: rounded to one
-//     it would add an error like P's own rounding, and so would K.
+//     it would add an error like P's own rounding, and so would K.  (V below 2^-14 is
+//     f16 subnormals, whose products the matrix core sums to 2^-18 only: f32 rows over V of
+//     3e-6 come out to 8e-7 where others do to 2.7e-7.  A common power of two as in
+//     the other kernel would have to be agreed on by the waves before they write V.)
 // For 64 keys and 16 columns at d 128 that is 48 MFMAs (768 cycles) and about 200
 // vector instructions (800 cycles), which do not run beside each other in one
 // wave, and the two waves of a SIMD meet at a barrier each 64 keys.  2048 rows

@@ -20,8 +20,8 @@ PATHS = [
     (1, 4, 128, 16, [1, 300, 33], [1, 5, 2], True),
     (2, 4, 96, 64, [1, 3000, 1, 2300], [1, 2, 1, 1], True),      # steps shared by workgroups
     (1, 2, 256, 16, [2100, 1], [1, 1], True),
-    (16, 16, 64, 16, [230, 233], [230, 233], True),              # the prompts' kernel
-    (16, 16, 128, 16, [230, 233], [230, 233], True),
+    (4, 64, 64, 16, [230, 233], [230, 233], True),              # the prompts' kernel
+    (4, 64, 128, 16, [230, 233], [230, 233], True),
 ]
 
 
@@ -134,8 +134,8 @@ def test_keys_that_are_alike(kv4, heads, group, d, page, lens, rows, causal, dty
 
 
 @pytest.mark.parametrize("top,scale", [(3e38, 2e-38), (1e36, 1e-36), (1e-36, 1e36)])
-@pytest.mark.parametrize("heads,group,d,page,lens,rows", [(16, 16, 64, 16, [230, 233], [230, 233]),
-                                                           (16, 16, 256, 16, [200, 217], [200, 217])])
+@pytest.mark.parametrize("heads,group,d,page,lens,rows", [(4, 64, 64, 16, [230, 233], [230, 233]),
+                                                           (4, 64, 256, 16, [200, 217], [200, 217])])
 def test_prompts_of_large_and_small_rows(kv4, heads, group, d, page, lens, rows, top, scale):
     """f32 rows up to the largest numbers and of the smallest, the scale bringing the scores back."""
     say(f"prompt rows of {top:g}, scale {scale:g}, d {d}")

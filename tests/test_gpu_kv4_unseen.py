@@ -21,16 +21,16 @@ CASES = [
     (2, 4, 64, 64, [5000, 40], [6, 7], 3, 0),              # steps shared by workgroups
     (1, 8, 128, 16, [4100, 2222], [5, 2], 2, 3000),
     (1, 3, 256, 128, [2500], [4], 1, 1700),
-    (16, 16, 64, 16, [230, 233], [230, 215], 200, 0),      # the prompts' kernel
-    (16, 16, 96, 16, [230, 233], [230, 215], 200, 0),
-    (16, 16, 128, 16, [230, 233], [230, 215], 200, 0),
-    (16, 16, 256, 16, [230, 233], [230, 215], 200, 0),
-    (16, 8, 64, 64, [400, 270], [250, 250], 250, 70),
-    (16, 16, 128, 64, [400, 270], [250, 250], 240, 81),
+    (4, 64, 64, 16, [230, 233], [230, 215], 200, 0),      # the prompts' kernel
+    (4, 64, 96, 16, [230, 233], [230, 215], 200, 0),
+    (4, 64, 128, 16, [230, 233], [230, 215], 200, 0),
+    (4, 64, 256, 16, [230, 233], [230, 215], 200, 0),
+    (4, 32, 64, 64, [400, 270], [250, 250], 250, 70),
+    (4, 64, 128, 64, [400, 270], [250, 250], 240, 81),
 ]
 
 
-@pytest.mark.parametrize("dtype,bits", [("f16", 0xffff), ("f32", 0x7c00), ("f32", 0x7c01)])
+@pytest.mark.parametrize("dtype,bits", [("f16", 0x7c00), ("f32", 0xffff)])
 @pytest.mark.parametrize("heads,group,d,page,lens,rows,kept,window", CASES)
 def test_unwritten_positions(kv4, heads, group, d, page, lens, rows, kept, window, dtype, bits):
     say(f"unwritten {heads}x{group}x{d} page {page} {lens} {rows} kept {kept} window {window} {dtype} {bits:#x}")
