@@ -45,6 +45,12 @@ inline bool kv4_on_batch(const madi_kv4_batch *b, const void *a, size_t an) {
   return kv4_overlap(a, an, b->table, (size_t)b->b * b->max_pages * 4) || kv4_overlap(a, an, b->lens, (size_t)b->b * 4) ||
          (b->row_off && kv4_overlap(a, an, b->row_off, ((size_t)b->b + 1) * 4));
 }
+// deferred_before_write for an extent of which a call writes some rows: what a recorded
+// dequantisation owes the rest is carried out first.
+inline int kv4_before_write(const void *p, size_t bytes) {
+  if (int rc = deferred_before_read(p, bytes)) return rc;
+  return deferred_before_write(p, bytes);
+}
 
 // ---------------------------------------------------------------- device side
 // A number that no kernel writes while others read it: at a uniform address one

@@ -339,11 +339,11 @@ int run(const char *what, const madi_kv4 *c, const madi_kv4_batch *b, void *k, v
   if (STORE) {
     if (int rc = deferred_before_read(k, kb)) return rc;
     if (int rc = deferred_before_read(v, vb)) return rc;
-    if (int rc = deferred_before_write(c->data, cb)) return rc;
+    if (int rc = kv4_before_write(c->data, cb)) return rc;
   } else {
     if (int rc = deferred_before_read(c->data, cb)) return rc;
-    if (int rc = deferred_before_write(k, kb)) return rc;
-    if (int rc = deferred_before_write(v, vb)) return rc;
+    if (int rc = kv4_before_write(k, kb)) return rc;
+    if (int rc = kv4_before_write(v, vb)) return rc;
   }
   const dim3 grid((uint32_t)gx, b->b);
   const bool f = dtype == MADI_F32;

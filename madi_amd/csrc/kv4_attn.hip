@@ -1374,7 +1374,7 @@ extern "C" int madi_kv4_attn(void *out, const void *q, const madi_kv4 *cache, co
     return fail(MADI_ERR_SHAPE, "%s: %u rows of %u sequences in one call", what, batch->rows, batch->b);
   if (int rc = deferred_before_read(q, qb)) return rc;
   if (int rc = deferred_before_read(cache->data, cb)) return rc;
-  if (int rc = deferred_before_write(out, ob)) return rc;
+  if (int rc = kv4_before_write(out, ob)) return rc;
   if (p.groups)
     if (int rc = deferred_before_write(batch->work, wb)) return rc;
   a.q = q;
