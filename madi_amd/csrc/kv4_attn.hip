@@ -50,6 +50,15 @@ constexpr int kKeys = 32;  // keys of a step
 constexpr int kPromptWaves = 8;
 constexpr int prompt_tiles(int d, bool f32) { return d < 128 || (d == 128 && !f32) ? 2 : 1; }
 constexpr int prompt_keys(int d) { return d == 256 ? 32 : 64; }
+// What a prompt's workgroup takes for 64 keys, in tenths of the time in which a CU's
+// sixteen waves of the other kernel take four steps.  Measured: 2048 rows of 4 heads of
+// d over one over 8192 keys, 4 of those, us here and there, f16 rows 260 and 356, 316 and 346,
+// 366 and 385, 525 and 653 (d 64, 96, 128, 256), f32 318 and 353, 413 and 396, 322 and 451.
+constexpr uint32_t prompt_cost(int d, bool f32) {
+  return f32 ? (d == 64 ? 36 : d == 96 ? 42 : 29) : d == 64 ? 29 : d == 96 ? 37 : d == 128 ? 38 : 31;
+}
+// f32 rows of 256 do not fit the registers (97 spilled): 1299 us there, 844 in the other kernel.
+constexpr bool has_prompt_kernel(int d, bool f32) { return d < 256 || !f32; }
 constexpr float kNever = -__FLT_MAX__;  // reference before any key was seen
 // P is 2^(x - M) with M at first the largest x - 7, raised when an x passes M
 // by 14: P at most 2^14, P s 2^-e at most 2^15 (f16 holds 2^16), and what
@@ -1267,17 +1276,15 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
   uint64_t len = b->len_max && b->len_max < reach ? b->len_max : reach;
   if (window && (uint64_t)window + b->rows + kKeys < len) len = (uint64_t)window + b->rows + kKeys;
   const uint64_t cols = (uint64_t)b->rows * (nh / c->nkv);
-  // Prompts where their workgroups fill the device.  One of them takes as long for
-  // 64 keys as a wave of the other kernel, of which a CU has 16 (four times as fast
-  // as one), for 5 * 4 of its steps with two tiles of columns per wave, 3 * 4 with
-  // one.  (2048 rows over 16384 keys, 32 heads of 128 over 8: 748 us here, 1411
-  // there; four of 17 to 224 rows over as many keys, 20 heads of 64, f32: 17.3 us here, 9.8 there.)
-  const uint64_t pcols = (uint64_t)kPromptWaves * 16 * prompt_tiles(c->d, dtype == MADI_F32);
+  // Prompts where their workgroups fill the device.  Times are counted in steps of a CU
+  // with sixteen waves of the other kernel (four steps at once), tenths of them.
+  const bool f32 = dtype == MADI_F32;
+  const uint64_t pcols = (uint64_t)kPromptWaves * 16 * prompt_tiles(c->d, f32);
   const uint64_t ptiles = (cols + pcols - 1) / pcols, steps = (len + kKeys - 1) / kKeys;
-  const uint64_t cost = (len + 63) / 64 * (prompt_tiles(c->d, dtype == MADI_F32) == 2 ? 5 : 3);
+  const uint64_t cost = (len + 63) / 64 * prompt_cost(c->d, f32);
   const uint64_t tiles16 = (cols + kCols - 1) / kCols * c->nkv * b->b;
   const uint64_t rounds = (ptiles * c->nkv * b->b + cus - 1) / cus;
-  if (!most && rounds * cost < tiles16 * steps / (4 * cus)) {
+  if (!most && has_prompt_kernel(c->d, f32) && rounds * cost < 10 * tiles16 * steps / (4 * cus)) {
     p.prompt = true;
     p.tiles = (uint32_t)ptiles;
     return p;
@@ -1299,9 +1306,11 @@ Plan plan_of(const madi_kv4 *c, const madi_kv4_batch *b, uint32_t nh, int dtype,
 
 template <int NB, typename T>
 void launch(const AttnArgs &a, const Plan &p, uint32_t cus) {
-  if (p.prompt) {
-    kv4_prompt_kernel<NB, T><<<a.items * a.kv.nkv, 64 * kPromptWaves, 0, stream()>>>(KV4_ARGS(a.kv), a);
-    return;
+  if constexpr (has_prompt_kernel(NB * 32, sizeof(T) == 4)) {
+    if (p.prompt) {
+      kv4_prompt_kernel<NB, T><<<a.items * a.kv.nkv, 64 * kPromptWaves, 0, stream()>>>(KV4_ARGS(a.kv), a);
+      return;
+    }
   }
   if (!p.groups) {
     constexpr int W = waves_alone(NB * 32, sizeof(T) == 4);
