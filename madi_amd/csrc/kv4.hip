@@ -11,11 +11,12 @@
 //
 // Both are bound by memory, K's and V's loads in flight together: 131072 rows
 // of 8 heads of 128 in f16 read back in 137 us (0.69 GB at 5.0 TB/s, where a copy
-// reaches 4.7: three quarters are writes), 16384 stored in 23.4 (3.7 TB/s: the codes'
+// reaches 5.1 to 5.24), 16384 stored in 23.2 (3.7 TB/s: the codes'
 // arithmetic is not all hidden behind the copy) and read back in
-// 15.4, single rows of eight sequences in 3.6 and 2.9, which is the latencies of a
+// 15.3, single rows of eight sequences in 3.3 and 2.7, which is the latencies of a
 // length, a page number and the rows, one after the other.  (Two units per lane: 130
-// us for the first, but 24 sequences' ragged prompts 17.8 in place of 13.8, stored and read.)
+// us for the first, but 24 sequences' ragged prompts, stored and read, 17.8 where they
+// took 13.8 then, 12.5 now.)
 #include "kv4.h"
 
 using namespace madi;

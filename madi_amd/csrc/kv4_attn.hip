@@ -24,12 +24,12 @@
 // f32 rows: q and P s are each split in two f16 (22 bits).
 //
 // What it costs (us, f16 rows, d 128; one MI355X):
-//   128 sequences of 8192, 32 heads over 8: 229, 1.21 GB at 5.3 TB/s of the 6.5
-//     that a kernel which only reads reaches.  A step of 32 keys is 326 vector
+//   128 sequences of 8192, 32 heads over 8: 226 to 229, 1.21 GB at 5.3 TB/s of the 6.5
+//     that a kernel which only reads reaches.  A step of 32 keys is 327 vector
 //     instructions (144 make codes of nibbles, 48 apply the K scales, 48 make P s)
-//     and 16 MFMAs: the vector pipe is busy 70 % of the time, the matrix pipe 14 %,
+//     and 16 MFMAs: the vector pipe is busy 68 % of the time, the matrix pipe 13 %,
 //     and 16 % of the waves' time is waiting for memory or barriers.
-//   1 sequence of 131072: 40.6, 33 in the kernel (4.6 TB/s; eight steps per wave
+//   1 sequence of 131072: 40.5, 33 in the kernel (4.6 TB/s; eight steps per wave
 //     do not hide a segment's beginning and end), 5.4 in the join.
 //   1 token over 213 keys, 20 heads of 64, f32: 5.7, of which 3 are launch and
 //     the rest five dependent memory latencies (length, pages, words, results in
@@ -70,7 +70,7 @@ constexpr float kLift = 7.0f, kRaise = 14.0f;
 // score itself as the reference M, without e, and raises it with every larger one: P is at
 // most 1, P s at most 9352.  A score is rounded before its reference is taken off, which
 // is exact then: a multiply-add would leave in what the rounding of the reference
-// took, 2^-24 of 10^10.  (Seven instructions more in 326; the longest caches' times are the same.)
+// took, 2^-24 of 10^10.  (327 vector instructions a step in place of 326, the same times.)
 constexpr float kFar = 0x1p20f;
 __device__ inline bool is_far(float limit) { return !(__builtin_fabsf(limit) < kFar); }
 
@@ -904,9 +904,9 @@ __global__ __launch_bounds__(TH) void kv4_attn_join_kernel(KV4_PARAMS, AttnArgs 
 // For 64 keys and 16 columns at d 128 that is 48 MFMAs (768 cycles) and about 200
 // vector instructions (800 cycles), which do not run beside each other in one
 // wave, and the two waves of a SIMD meet at a barrier each 64 keys.  2048 rows
-// over 16384 keys (causal, 32 heads of 128 over 8): 748 us, 689 TFLOP/s of the
+// over 16384 keys (causal, 32 heads of 128 over 8): 730 to 748 us, 689 to 706 TFLOP/s of the
 // product's 2 x 2 operations, the high and low V's third MFMA not counted (a
-// library f16 product of 8192^3 reaches 1168).  Two groups of waves, one multiplying while the
+// library f16 product of 8192^3 with a transposed operand sustains 1520).  Two groups of waves, one multiplying while the
 // other does its softmax, took 860.
 template <int NB, int KC>
 struct Buffer {
