@@ -466,7 +466,8 @@ __device__ inline void raise(Acc<NB> &A, const VScales<NB> &c, const float (&x)[
     big = max_across(big);
   }
   top = max_across(top);
-  if (top > A.limit) A.limit = is_far(top) ? top : top - kLift + kRaise;
+  // (a column whose M + kRaise would be far, M not: M = top - kRaise)
+  if (top > A.limit) A.limit = is_far(top - kLift + kRaise) ? top : top - kLift + kRaise;
   if (big > A.most) {
     const int e = __builtin_amdgcn_frexp_expf(big);
     A.e = (float)e;

@@ -192,3 +192,50 @@ def test_the_largest_scales(kv4, heads, group, d, page, lens, rows, causal, dtyp
     got = out.cpu().numpy().reshape(s.m, nh, d).astype(np.float64)
     assert np.all(np.isfinite(got))
     check(got[alone], want[alone], tol[alone], dtype)
+
+
+@pytest.mark.parametrize("score", [2.0 ** 20 - 20, 2.0 ** 20 - 10, 2.0 ** 20 - 3, 2.0 ** 20 + 4, -(2.0 ** 20) - 3, 2.0 ** 24,
+                                   2.0 ** 27 + 2.0 ** 20, -(2.0 ** 28)])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("heads,group,d,page,lens,rows,causal", PATHS[1:4])
+def test_small_values_under_large_scores(kv4, heads, group, d, page, lens, rows, causal, dtype, score):
+    """Keys that are alike with scores (as powers of 2) around 2^20 and past it, V of 10^-5
+    and 10^-6: its mean, to as many bits as elsewhere (test_gpu_kv4_values.py's bound)."""
+    say(f"small V, scores {score:g} {heads}x{group}x{d} {lens} {dtype}")
+    rng = np.random.default_rng(sum(lens) + 7)
+    s = Setup(kv4, rng, heads, d, page, lens, rows)
+    s.fill(rng)
+    code = rng.integers(1, 8, d)
+    for i, n in enumerate(lens):
+        kq, ks, vq, vs, there = s.held[i]
+        kq[:], ks[:] = code, 3.0
+        v = rng.uniform(0.2, 1, (n, heads, d)) * (1e-5 if i % 2 else 2e-6)
+        vq[:], vs[:] = R.quantise(v.astype(np.float32))
+        for t in range(n):
+            p, o = s.place(i, t)
+            for h in range(heads):
+                R.put(s.data, page, d, p, h, o, kq[t, h], ks[t, h], vq[t, h], vs[t, h])
+    s.dev.copy_(torch.from_numpy(s.data))
+    nh = heads * group
+    scale = 2.0 ** -8
+    while dtype == "f16" and abs(score) / (3.0 * code.sum() * scale * 1.4426950408889634) > 3e4:
+        scale *= 4
+    q = np.full((s.m, nh, d), score / (3.0 * code.sum() * scale * 1.4426950408889634)).astype(NP[dtype])
+    tq = torch.from_numpy(q.reshape(s.m, -1)).cuda()
+    s.batch.reserve(s.cache, nh)
+    out = torch.full_like(tq, 77.0)
+    kv4.kvAttn(out, tq, s.cache, s.batch, nh, causal=causal, scale=scale)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().reshape(s.m, nh, d).astype(np.float64)
+    for i, n in enumerate(lens):
+        v = R.value(s.held[i][2], s.held[i][3])
+        for r, pos in enumerate(R.rows_of(n, rows[i])):
+            k = pos + 1 if causal else n
+            if k <= 0:
+                continue
+            o, a = (x.repeat(group, 0) for x in (v[:k].mean(0), np.abs(v[:k]).mean(0)))
+            tol = ((2.0 ** -10 if dtype == "f16" else 3 * 2.0 ** -22) + 32 * 2.0 ** -23 + (n / 32 + 64) * 2.0 ** -24) * a
+            tol += 2.0 ** -11 * np.abs(o) + 2.0 ** -25 if dtype == "f16" else 2.0 ** -24 * np.abs(o)
+            tol += 7 * float(s.held[i][3].astype(np.float64).max()) * n * 2.0 ** -31
+            worst = (np.abs(got[s.off[i] + r] - o) / tol).max()
+            assert worst <= 1, (i, r, worst)
