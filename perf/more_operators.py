@@ -486,7 +486,7 @@ def run(st):
         kv4.kvFork(p, st["parent"], case["beams"])
         kv4.kvCopy(st["kv4"], st["copies"])
         return st["table"], st["lens"], st["refs"], st["cache"]
-    kv4.kvGrow(p, st["add"], copy=False)  # (pages held elsewhere are only read there)
+    kv4.kvGrow(p, st["add"])
     kv4.kvTrim(p, st["to"])
     return p.row_off, p.row_seq, p.row_pos, p.slot, st["table"], st["lens"], st["refs"]
 
