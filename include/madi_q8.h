@@ -460,15 +460,18 @@ typedef struct {
   int64_t *slot;     /* device, [m]: its page * page + its place there; -1 from there on (or on
                         a page that is not there) */
   uint32_t m;
+  uint32_t kept;     /* not 0: holders that are no sequences of the table only read (madi_kv4_grow) */
 } madi_kv4_rows;
 
 /* Appends add[i] tokens to every sequence i: lens grows, free pages (refs 0), the lowest
  * first, go to the sequences in order.  A sequence whose last page is not full and has
  * other holders gets a copy instead: `copies` says what madi_kv4_copy has to copy, in
  * every pool, before rows are stored; where all holders grow in one call, the last of them
- * keeps the page.  With copies NULL a sequence appends to its last page whoever else holds it: for
- * callers who know that nobody else appends there (prompts kept for later requests are only
- * read).  A sequence is left as it is, with no rows, where its table has no room for
+ * keeps the page.  With kept a last page that no other sequence has (at the same place of its row)
+ * is appended to as it is: for pages that are held elsewhere too, but only to be read, and no
+ * further than the sequence has them (prompts kept for later requests).  With copies NULL a sequence
+ * appends to its last page whoever else holds it: for callers who know that nobody else appends
+ * there.  A sequence is left as it is, with no rows, where its table has no room for
  * its tokens, or where the pages or the m rows do not suffice for it and the sequences before it
  * (one that needs no page needs none left).  page as in madi_kv4; b at most 65535. */
 int madi_kv4_grow(const madi_kv4_pages *pages, const uint32_t *add, const madi_kv4_rows *rows);

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void kv4_trim_kernel(Pages p, const uint32_t *
 struct Rows {
   uint32_t *row_off, *copies, *row_seq, *row_pos;
   int64_t *slot;
-  uint32_t m;
+  uint32_t m, kept;
 };
 
 constexpr uint32_t kGrow = 1024;         // threads, and sequences of a tile
@@ -222,7 +222,8 @@ __device__ inline Plan plan_of(const Pages &p) {
 }
 
 // One workgroup.  Sequences in tiles of 1024, thread t has sequence 1024 j + t of tile j.
-//  1. holders of a shared last page that grow: the last of them keeps it where all holders grow, the others get copies
+//  1. holders of a shared last page that grow: the last of them keeps it where all holders grow, the others get copies;
+//     with `kept`, one that no other sequence has is left to its sequence
 //  2. a tile's sums of the pages and rows asked for decide who grows; lengths and row offsets
 //  3. refs are looked through from page 0 for as many free pages as that takes, 16384 at a time
 //     (the first ones are asked for at the start: a page that is free then is so until it is given out)
@@ -234,7 +235,7 @@ enum Grow { kPlain, kMaps, kPlan };
 template <Grow MODE>
 __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t *__restrict__ add, Rows r) {
   constexpr bool MAPS = MODE == kMaps;
-  __shared__ uint32_t list[MODE == kPlan ? 1 : kGrow * kScan], lds[2][kGrow / 64];
+  __shared__ uint32_t list[MODE == kPlan ? 3 * kGrow : kGrow * kScan], lds[2][kGrow / 64], asking;
   __shared__ uint32_t offs[MAPS ? kGrow + 1 : 1], ends[MAPS ? kGrow : 1];
   const uint32_t tid = threadIdx.x, tiles = MAPS ? 1 : (p.b + kGrow - 1) / kGrow, mask = (1u << p.shift) - 1;
   if (MODE == kPlan && blockIdx.x) {
@@ -256,6 +257,46 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
   const uint32_t free = p.state[0];
   uint32_t is_free = MODE == kPlan ? 0 : look(p, tid * kScan);
 
+  // Those of `some` whose last page no other sequence has (at its place in the row): a wave looks for another one, 256
+  // rows at a time from the sequence's neighbours on.
+  const auto alone = [&](uint64_t some) {
+    uint32_t *who = list, *page = list + kGrow, *column = list + 2 * kGrow;
+    const uint32_t lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), chunks = (p.b + 63) / 64;
+    for (uint32_t t = 0; t < tiles; ++t) {
+      const bool mine = some >> t & 1;
+      if (tid == 0) asking = 0;
+      if (!__syncthreads_or(mine)) continue;
+      if (mine) {
+        const uint32_t i = t * kGrow + tid, len = length(p, i);
+        who[atomicAdd(&asking, 1u)] = tid;
+        column[tid] = len >> p.shift;
+        page[tid] = p.table[(size_t)i * p.max_pages + (len >> p.shift)];
+      }
+      __syncthreads();
+      for (uint32_t e = wave; e < asking; e += kGrow / 64) {
+        const uint32_t at = who[e], i = t * kGrow + at, q = page[at], c = column[at];
+        bool other = false;
+        for (uint32_t k = 0; k < chunks && !other; k += 4) {
+          uint32_t j[4], v[4];
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u) {
+            j[u] = (i / 64 + k + u) % chunks * 64 + lane;
+            v[u] = p.table[(size_t)(j[u] < p.b ? j[u] : i) * p.max_pages + c];
+          }
+          bool found = false;
+#pragma unroll
+          for (uint32_t u = 0; u < 4; ++u)
+            found |= v[u] == q && j[u] < p.b && j[u] != i && pages_of(length(p, j[u]), p.shift) > c;
+          other = __any(found);
+        }
+        if (!other && lane == 0) page[at] = kNone;
+      }
+      __syncthreads();
+      if (mine && page[tid] != kNone) some &= ~(1ull << t);
+    }
+    return some;
+  };
+
   uint64_t copy = 0;
   if (r.copies) {
     uint64_t shared = 0;
@@ -264,10 +305,10 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
       if (q < p.n_pages && p.refs[q] > 1) shared |= 1ull << t;
     }
     if (__syncthreads_or(shared != 0)) {
-      // through mark, which is 0 before and after: the last of a page's growing holders, then how many they are
-      const auto each = [&](auto f) {
+      // through mark, which is 0 before and after: how many of a page's holders grow, then the last of them
+      const auto each = [&](uint64_t who, auto f) {
         for (uint32_t t = 0; t < tiles; ++t)
-          if (shared >> t & 1) {
+          if (who >> t & 1) {
             const uint32_t i = t * kGrow + tid;
             f(t, i, last_page(i, seq(i)));
           }
@@ -277,20 +318,24 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
       const auto clear = [&](uint32_t, uint32_t, uint32_t q) {
         __hip_atomic_store(p.mark + q, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       };
-      each([&](uint32_t, uint32_t i, uint32_t q) {
-        __hip_atomic_fetch_max(p.mark + q, i + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      });
-      each([&](uint32_t t, uint32_t i, uint32_t q) {
-        if (load(q) != i + 1) copy |= 1ull << t;
-      });
-      each(clear);
-      each([&](uint32_t, uint32_t, uint32_t q) {
+      each(shared, [&](uint32_t, uint32_t, uint32_t q) {
         __hip_atomic_fetch_add(p.mark + q, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       });
-      each([&](uint32_t t, uint32_t, uint32_t q) {
+      each(shared, [&](uint32_t t, uint32_t, uint32_t q) {
         if (load(q) < p.refs[q]) copy |= 1ull << t;
       });
-      each(clear);
+      each(shared, clear);
+      const uint64_t whole = shared & ~copy;  // of whose page all holders grow
+      if (r.kept) copy &= ~alone(copy);
+      if (__syncthreads_or(whole != 0)) {
+        each(whole, [&](uint32_t, uint32_t i, uint32_t q) {
+          __hip_atomic_fetch_max(p.mark + q, i + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        });
+        each(whole, [&](uint32_t t, uint32_t i, uint32_t q) {
+          if (load(q) != i + 1) copy |= 1ull << t;
+        });
+        each(whole, clear);
+      }
     }
   }
 
@@ -491,7 +536,7 @@ extern "C" int madi_kv4_grow(const madi_kv4_pages *pages, const uint32_t *add, c
   if (int rc = disjoint(what, x)) return rc;
   if (int rc = not_ready(what)) return rc;
   if (int rc = ready(x)) return rc;
-  const Rows r{rows->row_off, rows->copies, rows->row_seq, rows->row_pos, rows->slot, rows->m};
+  const Rows r{rows->row_off, rows->copies, rows->row_seq, rows->row_pos, rows->slot, rows->m, rows->kept};
   const bool maps = m && (r.row_seq || r.row_pos || r.slot);
   // Few rows: one workgroup.  More: the plan's launches, 3 us more, with the pages and maps over all CUs.  (Measured with
   // a trim, one workgroup against the plan: 48 sequences of 20 rows 11.7 / 14.4 us, of 80 20.8 / 14.4; 256 of 16

@@ -217,7 +217,8 @@ class _Pages(ctypes.Structure):
 
 class _Rows(ctypes.Structure):
     _fields_ = [("row_off", ctypes.c_void_p), ("copies", ctypes.c_void_p), ("row_seq", ctypes.c_void_p),
-                ("row_pos", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("m", ctypes.c_uint32)]
+                ("row_pos", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("m", ctypes.c_uint32),
+                ("kept", ctypes.c_uint32)]
 
 
 class Pages:
@@ -251,10 +252,11 @@ class Pages:
         self.copies.fill_(-1)
         self._c = _Pages(ptr(refs), ptr(self.mark), ptr(self.state), ptr(table), ptr(lens), self.n_pages, page, b,
                          max_pages)
-        self._r = _Rows(ptr(self.row_off), ptr(self.copies), ptr(self.row_seq), ptr(self.row_pos), ptr(self.slot), m)
-        self._in_place = _Rows(ptr(self.row_off), None, ptr(self.row_seq), ptr(self.row_pos), ptr(self.slot), m)
-        self.addr, self.rows_addr = ctypes.addressof(self._c), ctypes.addressof(self._r)
-        self.in_place_addr = ctypes.addressof(self._in_place)
+        rows = lambda copies, kept: _Rows(ptr(self.row_off), copies, ptr(self.row_seq), ptr(self.row_pos), ptr(self.slot), m,
+                                          kept)
+        self._rows = {None: rows(ptr(self.copies), 1), True: rows(ptr(self.copies), 0), False: rows(None, 0)}  # by `copy`
+        self.addr = ctypes.addressof(self._c)
+        self.rows_addr = {copy: ctypes.addressof(r) for copy, r in self._rows.items()}
 
     def batch(self, rows: int, len_max: int = 0) -> Batch:
         """The Batch of the rows of a kvGrow, at most `rows` per sequence."""
@@ -312,12 +314,15 @@ def _numbers(t, shape, p, what):
     return _here(what, "the numbers", t, shape, x.i32, x.u32)
 
 
-def kvGrow(p: Pages, add, copy: bool = True) -> None:
+def kvGrow(p: Pages, add, copy: bool | None = None) -> None:
     """Room for add [b] more tokens in each sequence, and the maps of their rows.  A last page that
-    others hold is to be copied first (p.copies); with copy False it is appended to as
-    it is, and p.copies stays what the grow before left there: for pages that nobody else
-    appends to, with no kvCopy after it."""
-    calls.madi_kv4_grow(p.addr, _numbers(add, (p.b,), p, "kvGrow"), p.rows_addr if copy else p.in_place_addr)
+    another sequence has too is to be copied first (p.copies).  What is held elsewhere (prompts kept for later
+    requests) is taken to be read only, and no further than the sequence has it: a page that is held
+    by one sequence and elsewhere is appended to.  With copy True such pages are copied too (a
+    sequence that was cut down to less than is kept of it needs that); with copy False no page is, and
+    p.copies stays what the grow before left there: for pages that nobody else appends to,
+    with no kvCopy after it."""
+    calls.madi_kv4_grow(p.addr, _numbers(add, (p.b,), p, "kvGrow"), p.rows_addr[copy])
 
 
 def kvTrim(p: Pages, to) -> None:
