@@ -466,8 +466,8 @@ typedef struct {
 /* Appends add[i] tokens to every sequence i: lens grows, free pages (refs 0), the lowest
  * first, go to the sequences in order.  A sequence whose last page is not full and has
  * other holders gets a copy instead: `copies` says what madi_kv4_copy has to copy, in
- * every pool, before rows are stored; where all holders grow in one call, the last of them
- * keeps the page.  With kept a last page that no other sequence has (at the same place of its row)
+ * every pool, before rows are stored; where all holders grow in one call, the one with the most
+ * tokens there (of equals the last) keeps the page, so that one that is left out loses none.  With kept a last page that no other sequence has (at the same place of its row)
  * is appended to as it is: for pages that are held elsewhere too, but only to be read, and no
  * further than the sequence has them (prompts kept for later requests).  With copies NULL a sequence
  * appends to its last page whoever else holds it: for callers who know that nobody else appends

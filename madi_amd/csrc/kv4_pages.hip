@@ -222,8 +222,9 @@ __device__ inline Plan plan_of(const Pages &p) {
 }
 
 // One workgroup.  Sequences in tiles of 1024, thread t has sequence 1024 j + t of tile j.
-//  1. holders of a shared last page that grow: the last of them keeps it where all holders grow, the others get copies;
-//     with `kept`, one that no other sequence has is left to its sequence
+//  1. holders of a shared last page that grow: where all holders do, the one with the most tokens in it keeps it, the
+//     others get copies (one that finds no page for its copy goes on holding the page, and no row of a longer one's is
+//     written where it has tokens); with `kept`, a page that no other sequence has is left to its sequence
 //  2. a tile's sums of the pages and rows asked for decide who grows; lengths and row offsets
 //  3. refs are looked through from page 0 for as many free pages as that takes, 16384 at a time
 //     (the first ones are asked for at the start: a page that is free then is so until it is given out)
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
       if (q < p.n_pages && p.refs[q] > 1) shared |= 1ull << t;
     }
     if (__syncthreads_or(shared != 0)) {
-      // through mark, which is 0 before and after: how many of a page's holders grow, then the last of them
+      // through mark, which is 0 before and after: how many of a page's holders grow, then the longest of them
       const auto each = [&](uint64_t who, auto f) {
         for (uint32_t t = 0; t < tiles; ++t)
           if (who >> t & 1) {
@@ -328,13 +329,24 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
       const uint64_t whole = shared & ~copy;  // of whose page all holders grow
       if (r.kept) copy &= ~alone(copy);
       if (__syncthreads_or(whole != 0)) {
-        each(whole, [&](uint32_t, uint32_t i, uint32_t q) {
-          __hip_atomic_fetch_max(p.mark + q, i + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        });
-        each(whole, [&](uint32_t t, uint32_t i, uint32_t q) {
-          if (load(q) != i + 1) copy |= 1ull << t;
-        });
-        each(whole, clear);
+        const auto tokens = [&](uint32_t i) { return length(p, i) & mask; };  // (at least one)
+        const auto most = [&](auto number) {  // keeps the page, so far; the others copy
+          const uint64_t left = whole & ~copy;
+          each(left, [&](uint32_t, uint32_t i, uint32_t q) {
+            __hip_atomic_fetch_max(p.mark + q, number(i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          });
+          each(left, [&](uint32_t t, uint32_t i, uint32_t q) {
+            if (load(q) != number(i)) copy |= 1ull << t;
+          });
+          each(left, clear);
+        };
+        // of equals the last: one number (sequences are 2^16 - 1 at most), or two for pages of more than 2^16 tokens
+        if (p.shift <= 16) {
+          most([&](uint32_t i) { return tokens(i) << 16 | i; });
+        } else {
+          most(tokens);
+          most([&](uint32_t i) { return i + 1; });
+        }
       }
     }
   }

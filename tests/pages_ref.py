@@ -23,7 +23,7 @@ class Pages(S.Pages):
         for i, p in last.items():
             grow = [j for j in last if last[j] == p]
             if len(grow) == before[p]:
-                if i != grow[-1]:
+                if i != max(grow, key=lambda j: (self.length(j) % self.page, j)):
                     out.add(i)
             elif before[p] > 1 and (copy or len(self.sequences(p, self.length(i) // self.page)) > 1):
                 out.add(i)
@@ -62,3 +62,48 @@ class Pages(S.Pages):
             q = int(self.table[i, p // self.page])
             seq[r], pos[r], slot[r] = i, p, q * self.page + p % self.page if self.there(q) else NONE
         return np.array(row_off, np.int32), out, seq, pos, slot
+
+
+class Contents:
+    """What the pages hold: a number for every token that a sequence was given, written where a grow
+    says and copied as it says."""
+
+    def __init__(self, n_pages, page, b):
+        self.pool, self.page = np.zeros((n_pages, page), np.int64), page
+        self.tokens, self.given = [[] for _ in range(b)], 0
+
+    def grow(self, copies, seq, slot):
+        for source, to, n in copies:
+            if source != NONE:
+                self.pool[to, :n] = self.pool[source, :n]
+        for i, at in zip(seq, slot):
+            if i != NONE:
+                self.given += 1
+                self.pool.reshape(-1)[at] = self.given
+                self.tokens[i].append(self.given)
+
+    def trim(self, to):
+        self.tokens = [t[:n] for t, n in zip(self.tokens, to)]
+
+    def fork(self, parent, beams):
+        self.tokens = [list(self.tokens[i // beams * beams + parent[i // beams, i % beams]]) for i in range(len(self.tokens))]
+
+    def check(self, table, lens):
+        for i, tokens in enumerate(self.tokens):
+            at = np.arange(int(lens[i]))
+            assert self.pool[table[i, at // self.page], at % self.page].tolist() == tokens, i
+
+
+def holders_of_many_lengths(rng, b, beams, page, max_pages, m, steps):
+    """Steps after which last pages have holders of different lengths: (name, argument) one after the other.  `lens`
+    is sent in before each."""
+    lens = yield
+    for step in range(steps):
+        lens = yield "grow", (rng.random(b) < (1, 0.8, 0.5)[step % 3]) * rng.integers(1, 4, b)
+        if step % 5 == 4:
+            lens = yield "grow", np.where(np.arange(b) == rng.integers(b), rng.integers(0, m // 2 + 1), 1)
+        # cut down within the last page, mostly; some are ended
+        to = np.maximum(lens - (rng.random(b) < 0.4) * rng.integers(0, page // 2, b), 0)
+        lens = yield "trim", np.where(rng.random(b) < 0.05, 0, to)
+        if step % 2:
+            lens = yield "fork", rng.integers(0, beams, (b // beams, beams))

@@ -114,6 +114,70 @@ def test_kept_prompts_and_beams(kv4, groups, beams, max_pages, m):
     t.grow((rng.random(b) < 0.6).astype(int), copy=True)
 
 
+def contents(kv4, n_pages, page, b, max_pages, m):
+    """Both with what the pages hold; the GPU's tables, copies and slots say where."""
+    t, held = Both(kv4, n_pages, page, b, max_pages, m), pages_ref.Contents(n_pages, page, b)
+
+    def take(name, arg, copy=None):
+        arg = np.asarray(arg)
+        if name == "grow":
+            t.grow(arg, copy)
+            held.grow(*(getattr(t.gpu, x).cpu().numpy() for x in ("copies", "row_seq", "slot")))
+        else:
+            for x in (t, held):
+                x.fork(arg, arg.shape[1]) if name == "fork" else x.trim(arg)
+        held.check(t.gpu.table.cpu().numpy(), t.gpu.lens.cpu().numpy())
+    return t, take
+
+
+@pytest.mark.parametrize("copy", [None, True])
+@pytest.mark.parametrize("m", [9, 5000])
+def test_a_sequence_that_is_left_out_keeps_its_tokens(kv4, m, copy):
+    """The one that would copy finds no page, a shorter one asks for the page as well: the longer keeps it."""
+    t, take = contents(kv4, 2, 16, 3, 2, m)
+    for name, arg in (("grow", [5, 0, 0]), ("fork", [[0, 0, 0]]), ("grow", [1, 1, 1]), ("fork", [[0, 2, 1]]), ("grow", [0, 1, 1])):
+        take(name, arg, copy)
+    assert t.ref.lens.tolist() == [6, 7, 5] and t.ref.left_out == 1
+    t, take = contents(kv4, 1, 16, 3, 2, m)
+    for name, arg in (("grow", [6, 0, 0]), ("fork", [[0, 0, 0]]), ("trim", [9, 0, 3]), ("grow", [1, 0, 1])):
+        take(name, arg, copy)
+    assert t.ref.lens.tolist() == [7, 0, 3] and t.ref.left_out == 1
+
+
+@pytest.mark.parametrize("groups,beams,page,share,m", [(1, 3, 16, 0.7, 9), (5, 4, 16, 0.7, 40), (5, 4, 32, 1.2, 4000), (60, 5, 16, 0.6, 500),
+                                                       (60, 5, 16, 0.8, 9000), (275, 4, 16, 0.8, 2000), (275, 4, 64, 0.7, 15000)])
+def test_holders_of_many_lengths(kv4, groups, beams, page, share, m):
+    """Sequences cut down, forked and grown in any number, in pools that run short; one workgroup and the plan's."""
+    rng = np.random.default_rng(groups * beams + m)
+    b = groups * beams
+    t, take = contents(kv4, int(b * share) + 1, page, b, 4, m)
+    steps = pages_ref.holders_of_many_lengths(rng, b, beams, page, 4, m, 12 if b < 500 else 6)
+    next(steps)
+    while True:
+        try:
+            name, arg = steps.send(t.ref.lens)
+        except StopIteration:
+            break
+        take(name, arg, None if rng.random() < 0.7 else True)
+
+
+def test_pages_of_many_tokens(kv4):
+    """Pages too large for a sequence's length and number to share a word: the longest keeps it, of equals the last."""
+    for page in (1 << 16, 1 << 17, 1 << 20):
+        n = page - 3
+        t = Both(kv4, 8, page, 4, 2, m=page)
+        t.grow([n, 0, 0, 0])
+        t.fork([[0, 0, 0, 0]], 4)
+        t.trim([n, n, n - 1, 5])
+        assert (t.grow([1, 1, 1, 1])[:, 0] >= 0).tolist() == [True, False, True, True]
+        t.fork([[1, 1, 1, 1]], 4)
+        t.trim([n + 1, 1, 1 << 16 if page > 1 << 16 else 2, 1])
+        assert (t.grow([0, 1, 1, 1])[:, 0] >= 0).tolist() == [False, True, True, True]
+        t.trim([0, n, n, n])
+        t.fork([[0, 2, 2, 2]], 4)
+        assert (t.grow([0, 1, 1, 1])[:, 0] >= 0).tolist() == [False, True, True, False]
+
+
 @pytest.fixture
 def cases():
     from perf import more_operators
