@@ -5,6 +5,7 @@
 // kernels, whose sums start from B h.
 #include "kv4.h"
 #include "lora.h"
+#include "lora_places.h"
 
 using namespace madi;
 
@@ -179,12 +180,10 @@ __global__ __launch_bounds__(kTileWaves * 64) void lora_tile_kernel(Adapters l, 
   const uint32_t xr = m0 + wave < m ? m0 + wave : m - 1;
   const float *x = in + (size_t)xr * k;
   f32x4 v[kLoads];
-  const auto load_x = [&](uint32_t k0) {  // (past the row's end its first elements again: a branch per load, and a wait
+  const auto load_x = [&](uint32_t k0) {  // (past the row's end its last elements again: a branch per load, and a wait
 #pragma unroll                            //  for all loads and stores before each use, took 3 us more)
-    for (uint32_t j = 0; j < kLoads; ++j) {
-      const uint32_t at = k0 + j * 256 + lane * 4;
-      v[j] = *reinterpret_cast<const f32x4 *>(x + (at < k ? at : lane * 4));
-    }
+    for (uint32_t j = 0; j < kLoads; ++j)
+      v[j] = *reinterpret_cast<const f32x4 *>(x + lora_x_place(k0 + j * 256 + lane * 4, k));
   };
   load_x(0);
   const uint32_t mine = m0 + c < m ? adapter_of(l, row) : kNoAdapter;
