@@ -789,7 +789,7 @@ extern "C" int madi_beam_gather(const madi_beam_states *s) {
   if (s->ldp < s->beams) return fail(MADI_ERR_SHAPE, "%s: rows of parent are %u apart but %u long", what, s->ldp, s->beams);
   if (s->n_states > kMaxBeams) return fail(MADI_ERR_SHAPE, "%s: %u states (at most 32)", what, s->n_states);
   if (s->row_bytes % 4 || s->stride % 4) return fail(MADI_ERR_ALIGN, "%s: stride and row_bytes must be multiples of 4", what);
-  if (s->row_bytes > (1ull << 40) || s->stride > (1ull << 40) || s->rows * s->row_bytes > s->stride)
+  if (s->row_bytes > (1ull << 40) || s->stride > (1ull << 40) || (s->rows && s->row_bytes > s->stride / s->rows))
     return fail(MADI_ERR_SHAPE, "%s: %u rows of %zu bytes, states %zu bytes apart", what, s->rows, s->row_bytes, s->stride);
   const size_t bytes = (size_t)s->rows * s->row_bytes, slots = (size_t)s->groups * s->beams;
   if (!s->parent || (s->n_states && !s->dst)) return fail(MADI_ERR_NULL, "%s: null pointer", what);
