@@ -55,6 +55,7 @@ class Search:
         self.parent = torch.empty(groups, n, dtype=torch.int32, device=device)
         self.token = torch.empty(groups, n, dtype=torch.int32, device=device)
         self.work = torch.empty(need, dtype=torch.uint8, device=device)
+        self.on = _on("beam.Search", self.work)
         self._c = _Beam(None, None, None, None, 0, 0, groups, beams, vocab, n, eos, F32, ptr(self.score),
                         ptr(self.parent), ptr(self.token), ptr(self.work), need)
         self.addr = ctypes.addressof(self._c)
@@ -69,6 +70,8 @@ def beamSelect(s: Search, logits, score, done=None, ban=None) -> None:
     words = (vocab + 31) // 32, bit v % 32 of word v // 32 for each token v left out."""
     what, m, t = "beamSelect", s.groups * s.beams, _torch()
     device = DEVICE
+    if s.on and lib().madi_device_cu_count():
+        raise MadiError(-9, what, f"the Search must be in the memory of GPU {DEVICE}, is on {s.work.device}")
     r = t.rows(logits, m, s.vocab, t.f16, t.f32, device) if logits.dim() == 2 and logits.shape[0] == m else -1
     if r == -2 and not lib().madi_device_cu_count():  # (the library refuses the call by itself)
         device, r = -1, t.rows(logits, m, s.vocab, t.f16, t.f32, -1)

@@ -13,7 +13,7 @@ from __future__ import annotations
 import ctypes
 
 from ._lib import MadiError, calls, lib
-from .kv4 import _here, _torch
+from .kv4 import DEVICE, _here, _on, _torch
 from .q8 import Q8, ptr
 
 
@@ -41,6 +41,7 @@ class Adapters:
         at = (_here("lora.Adapters", "a", a, a.shape, t.f16, t.f16), _here("lora.Adapters", "b", b, b.shape, t.f16, t.f16),
               _here("lora.Adapters", "scale", scale, (self.n,), t.f32, t.f32))
         self.a, self.b, self.scale, self.work = a, b, scale, None
+        self.on = _on("lora.Adapters", a, b, scale)
         self._outgrown: list = []
         self.rows = 0  # that the workspace is enough for
         self._c = _Lora(*at, None, None, self.n, self.rank, 0, None, 0)
@@ -70,6 +71,8 @@ def pprojLora(in_f32, w: Q8, out_f32, M: int, N: int, Kk: int, ad: Adapters, ada
     what, t = "pprojLora", _torch()
     if Kk != ad.k or N != ad.width:
         raise MadiError(-5, what, f"adapters of {ad.k} -> {ad.width} for a projection of {Kk} -> {N}")
+    if ad.on and lib().madi_device_cu_count():
+        raise MadiError(-9, what, f"the Adapters must be in the memory of GPU {DEVICE}, are on {ad.a.device}")
     x, y = _here(what, "in_f32", in_f32, (M, Kk), t.f32, t.f32), _here(what, "out_f32", out_f32, (M, N), t.f32, t.f32)
     c = ad._c
     if row_seq is None:
