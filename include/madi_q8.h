@@ -541,7 +541,8 @@ int madi_beam_gather(const madi_beam_states *states);
 /* ---- low-rank adapters ------------------------------------------------------------ */
 /* madi_q8_pproj with an adapter for each row (no counterpart in the reference):
  *   out[m] = W x + scale[a] B[a] (A[a] x),  x = f16(in[m]), W = f16(q s), a the row's adapter
- * A and B f16, every sum f32 and A x kept to 22 bits or more; a row whose adapter is `adapters` or more has
+ * A and B f16, every sum f32 and A x kept to 22 bits or more (an infinite one as it is; an
+ * infinity in B may make its outputs NaN); a row whose adapter is `adapters` or more has
  * none, and is what madi_q8_pproj gives (from 512 rows on but for the order of its sums).  a = adapter[m], or adapter[row_seq[m]] with
  * the rows' sequences (madi_kv4_rows; one of `seqs` or more: none).  rank: a multiple of 8,
  * 8 to 128 (smaller ones filled up with zeros).  Where madi_q8_pproj splits K over workgroups

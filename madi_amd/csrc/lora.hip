@@ -52,17 +52,21 @@ __device__ inline float wave_sum(float v) {
   return __builtin_bit_cast(float, (uint32_t)y[0]) + __builtin_bit_cast(float, (uint32_t)y[1]);
 }
 
-// A row's h as two f16: the largest is scaled to 2^14 .. 2^15, where the low part of every value that
-// counts is a normal f16.
+// A row's h as two f16: the largest (of those that are finite) is scaled to 2^14 .. 2^15, where the low part of every
+// value that counts is a normal f16.  An infinity is one in the high part alone: B h is what it is in f32.
+__device__ inline float finite(float v) {
+  v = __builtin_fabsf(v);
+  return v < INFINITY ? v : 0.0f;
+}
 __device__ inline int exponent_of(float top) {
-  if (!(top > 0) || !(top < INFINITY)) return 0;
+  if (!(top > 0)) return 0;
   const int e = __builtin_amdgcn_frexp_expf(top) - 15;
   return e < -126 ? -126 : e;
 }
 __device__ inline void halves(float v, int e, f16 &hi, f16 &lo) {
   v = __builtin_amdgcn_ldexpf(v, -e);
   hi = (f16)v;
-  lo = (f16)(v - (float)hi);
+  lo = __builtin_fabsf(v) < INFINITY ? (f16)(v - (float)hi) : (f16)0.0f;
 }
 
 // The XCDs take workgroups in turn: here each gets neighbours, whose rows mostly share an adapter that its L2 reads
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(1024) void lora_row_kernel(Adapters l, const float 
   if (threadIdx.x < l.rank) {
     float top = 0;
 #pragma unroll 8
-    for (uint32_t r = 0; r < l.rank; ++r) top = __builtin_fmaxf(top, __builtin_fabsf(hs[r]));
+    for (uint32_t r = 0; r < l.rank; ++r) top = __builtin_fmaxf(top, finite(hs[r]));
     const int e = exponent_of(top);
     const LoraShape shape = lora_shape(l.rank, tile_rows);
     halves(hs[threadIdx.x], e, h[lora_at(shape, row, threadIdx.x, false)], h[lora_at(shape, row, threadIdx.x, true)]);
@@ -277,7 +281,7 @@ __global__ __launch_bounds__(kTileWaves * 64) void lora_tile_kernel(Adapters l, 
     // (ranks come in eights; numbers at least 0 are in the order of their bits)
     float top = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top = __builtin_fmaxf(top, __builtin_fabsf(sum[e]));
+    for (int e = 0; e < 4; ++e) top = __builtin_fmaxf(top, finite(sum[e]));
     if (r0 < l.rank) atomicMax(&tops[c], __builtin_bit_cast(uint32_t, top));
   }
   __syncthreads();
