@@ -221,6 +221,11 @@ __device__ inline Plan plan_of(const Pages &p) {
   return {first, first + p.b + 1, first + p.b + 1 + segments(p.n_pages)};
 }
 
+// A sequence whose last page has other holders.
+struct Sharer {
+  uint32_t seq, page, len, held, yes;
+};
+
 // One workgroup.  Sequences in tiles of 1024, thread t has sequence 1024 j + t of tile j.
 //  1. holders of a shared last page that grow: where all holders do, the one with the most tokens in it keeps it, the
 //     others get copies (one that finds no page for its copy goes on holding the page, and no row of a longer one's is
@@ -236,7 +241,7 @@ enum Grow { kPlain, kMaps, kPlan };
 template <Grow MODE>
 __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t *__restrict__ add, Rows r) {
   constexpr bool MAPS = MODE == kMaps;
-  __shared__ uint32_t list[MODE == kPlan ? 3 * kGrow : kGrow * kScan], lds[2][kGrow / 64], asking;
+  __shared__ uint32_t list[MODE == kPlan ? kGrow * sizeof(Sharer) / 4 : kGrow * kScan], lds[2][kGrow / 64], asking;
   __shared__ uint32_t offs[MAPS ? kGrow + 1 : 1], ends[MAPS ? kGrow : 1];
   const uint32_t tid = threadIdx.x, tiles = MAPS ? 1 : (p.b + kGrow - 1) / kGrow, mask = (1u << p.shift) - 1;
   if (MODE == kPlan && blockIdx.x) {
@@ -258,54 +263,72 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
   const uint32_t free = p.state[0];
   uint32_t is_free = MODE == kPlan ? 0 : look(p, tid * kScan);
 
-  // Those of `some` whose last page no other sequence has (at its place in the row): a wave looks for another one, 256
-  // rows at a time from the sequence's neighbours on.
-  const auto alone = [&](uint64_t some) {
-    uint32_t *who = list, *page = list + kGrow, *column = list + 2 * kGrow;
-    const uint32_t lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), chunks = (p.b + 63) / 64;
-    for (uint32_t t = 0; t < tiles; ++t) {
-      const bool mine = some >> t & 1;
-      if (tid == 0) asking = 0;
-      if (!__syncthreads_or(mine)) continue;
-      if (mine) {
-        const uint32_t i = t * kGrow + tid, len = length(p, i);
-        who[atomicAdd(&asking, 1u)] = tid;
-        column[tid] = len >> p.shift;
-        page[tid] = p.table[(size_t)i * p.max_pages + (len >> p.shift)];
-      }
-      __syncthreads();
-      for (uint32_t e = wave; e < asking; e += kGrow / 64) {
-        const uint32_t at = who[e], i = t * kGrow + at, q = page[at], c = column[at];
-        bool other = false;
-        for (uint32_t k = 0; k < chunks && !other; k += 4) {
-          uint32_t j[4], v[4];
+  // Whether another sequence than i has page q as number c of its own: a wave looks, 256 rows at a time from i's
+  // neighbours on.
+  const uint32_t lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const auto another = [&](uint32_t i, uint32_t q, uint32_t c) {
+    const uint32_t chunks = (p.b + 63) / 64;
+    for (uint32_t k = 0; k < chunks; k += 4) {
+      uint32_t j[4], v[4];
 #pragma unroll
-          for (uint32_t u = 0; u < 4; ++u) {
-            j[u] = (i / 64 + k + u) % chunks * 64 + lane;
-            v[u] = p.table[(size_t)(j[u] < p.b ? j[u] : i) * p.max_pages + c];
-          }
-          bool found = false;
-#pragma unroll
-          for (uint32_t u = 0; u < 4; ++u)
-            found |= v[u] == q && j[u] < p.b && j[u] != i && pages_of(length(p, j[u]), p.shift) > c;
-          other = __any(found);
-        }
-        if (!other && lane == 0) page[at] = kNone;
+      for (uint32_t u = 0; u < 4; ++u) {
+        j[u] = (i / 64 + k + u) % chunks * 64 + lane;
+        v[u] = p.table[(size_t)(j[u] < p.b ? j[u] : i) * p.max_pages + c];
       }
-      __syncthreads();
-      if (mine && page[tid] != kNone) some &= ~(1ull << t);
+      bool found = false;
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u)
+        found |= v[u] == q && j[u] < p.b && j[u] != i && pages_of(length(p, j[u]), p.shift) > c;
+      if (__any(found)) return true;
     }
-    return some;
+    return false;
+  };
+  // The sequences of the threads with `mine` side by side in LDS, f(e, n) of each of the n by a wave, and what that says.
+  Sharer *sharers = reinterpret_cast<Sharer *>(list);
+  const auto ask_of = [&](bool mine, const Sharer &own, auto f) {
+    if (tid == 0) asking = 0;
+    if (!__syncthreads_or(mine)) return false;
+    uint32_t at = 0;
+    if (mine) {
+      at = atomicAdd(&asking, 1u);
+      sharers[at] = own;
+    }
+    __syncthreads();
+    const uint32_t n = asking;
+    for (uint32_t e = wave; e < n; e += kGrow / 64) {
+      const bool yes = f(e, n);
+      if (lane == 0) sharers[e].yes = yes;
+    }
+    __syncthreads();
+    return mine && sharers[at].yes;
   };
 
   uint64_t copy = 0;
   if (r.copies) {
     uint64_t shared = 0;
+    Sharer own{};  // of the last tile
     for (uint32_t t = 0; t < tiles; ++t) {
-      const uint32_t i = t * kGrow + tid, q = last_page(i, seq(i));
-      if (q < p.n_pages && p.refs[q] > 1) shared |= 1ull << t;
+      const uint32_t i = t * kGrow + tid;
+      const Seq s = seq(i);
+      const uint32_t q = last_page(i, s), held = q < p.n_pages ? p.refs[q] : 0;
+      own = {i, q, s.len, held, 0};
+      if (held > 1) shared |= 1ull << t;
     }
-    if (__syncthreads_or(shared != 0)) {
+    if (tiles == 1) {
+      // one tile: a wave counts a sharer's page among the others (through mark it took 4 us more for 48 sequences)
+      copy = ask_of(shared, own, [&](uint32_t e, uint32_t n) {
+        const Sharer s = sharers[e];
+        uint32_t grow = 0;
+        bool most = true;
+        for (uint32_t x = lane; x - lane < n; x += 64) {
+          const Sharer o = sharers[x < n ? x : e];
+          const bool same = x < n && o.page == s.page;
+          grow += __builtin_popcountll(__ballot(same));
+          most &= !same || (o.len & mask) < (s.len & mask) || ((o.len & mask) == (s.len & mask) && o.seq <= s.seq);
+        }
+        return grow < s.held ? !r.kept || another(s.seq, s.page, s.len >> p.shift) : !__all(most);
+      });
+    } else if (__syncthreads_or(shared != 0)) {
       // through mark, which is 0 before and after: how many of a page's holders grow, then the longest of them
       const auto each = [&](uint64_t who, auto f) {
         for (uint32_t t = 0; t < tiles; ++t)
@@ -327,7 +350,17 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
       });
       each(shared, clear);
       const uint64_t whole = shared & ~copy;  // of whose page all holders grow
-      if (r.kept) copy &= ~alone(copy);
+      if (r.kept)
+        for (uint32_t t = 0; t < tiles; ++t) {
+          const bool mine = copy >> t & 1;
+          const uint32_t i = t * kGrow + tid;
+          const Seq its = seq(i);
+          const bool yes = ask_of(mine, {i, last_page(i, its), its.len, 0, 0}, [&](uint32_t e, uint32_t) {
+            const Sharer s = sharers[e];
+            return another(s.seq, s.page, s.len >> p.shift);
+          });
+          if (mine && !yes) copy &= ~(1ull << t);
+        }
       if (__syncthreads_or(whole != 0)) {
         const auto tokens = [&](uint32_t i) { return length(p, i) & mask; };  // (at least one)
         const auto most = [&](auto number) {  // keeps the page, so far; the others copy
