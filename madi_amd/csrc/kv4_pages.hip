@@ -225,6 +225,10 @@ __device__ inline Plan plan_of(const Pages &p) {
 struct Sharer {
   uint32_t seq, page, len, held, yes;
 };
+// Up to so many of them find one another in LDS, at a cost that goes with their square; more through mark's six phases.  (A
+// step of as many beams: 40 8.6 / 10.8 us, 128 10.7 / 11.0, 192 12.1 / 11.4, 800 50 / 16; 48 sequences, two of them on kept
+// prompts' pages, 10.0 / 12.0.)
+constexpr uint32_t kFew = 128;
 
 // One workgroup.  Sequences in tiles of 1024, thread t has sequence 1024 j + t of tile j.
 //  1. holders of a shared last page that grow: where all holders do, the one with the most tokens in it keeps it, the
@@ -285,9 +289,8 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
   };
   // The sequences of the threads with `mine` side by side in LDS, f(e, n) of each of the n by a wave, and what that says.
   Sharer *sharers = reinterpret_cast<Sharer *>(list);
+  // (asking is 0)
   const auto ask_of = [&](bool mine, const Sharer &own, auto f) {
-    if (tid == 0) asking = 0;
-    if (!__syncthreads_or(mine)) return false;
     uint32_t at = 0;
     if (mine) {
       at = atomicAdd(&asking, 1u);
@@ -314,8 +317,9 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
       own = {i, q, s.len, held, 0};
       if (held > 1) shared |= 1ull << t;
     }
-    if (tiles == 1) {
-      // one tile: a wave counts a sharer's page among the others (through mark it took 4 us more for 48 sequences)
+    if (tid == 0) asking = 0;
+    const uint32_t some = __syncthreads_count(shared != 0);
+    if (some && some <= kFew && tiles == 1) {  // a wave counts a sharer's page among the others
       copy = ask_of(shared, own, [&](uint32_t e, uint32_t n) {
         const Sharer s = sharers[e];
         uint32_t grow = 0;
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
         }
         return grow < s.held ? !r.kept || another(s.seq, s.page, s.len >> p.shift) : !__all(most);
       });
-    } else if (__syncthreads_or(shared != 0)) {
+    } else if (some) {
       // through mark, which is 0 before and after: how many of a page's holders grow, then the longest of them
       const auto each = [&](uint64_t who, auto f) {
         for (uint32_t t = 0; t < tiles; ++t)
@@ -354,6 +358,8 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
         for (uint32_t t = 0; t < tiles; ++t) {
           const bool mine = copy >> t & 1;
           const uint32_t i = t * kGrow + tid;
+          if (tid == 0) asking = 0;
+          if (!__syncthreads_or(mine)) continue;
           const Seq its = seq(i);
           const bool yes = ask_of(mine, {i, last_page(i, its), its.len, 0, 0}, [&](uint32_t e, uint32_t) {
             const Sharer s = sharers[e];
