@@ -190,6 +190,10 @@ __device__ inline Seq seq_of(const Pages &p, const uint32_t *add, uint32_t i) {
   }
   return s;
 }
+// The page that its next token goes to, if it has one.
+__device__ inline uint32_t last_page(const Pages &p, uint32_t i, const Seq &s) {
+  return s.add && (s.len & ((1u << p.shift) - 1)) ? p.table[(size_t)i * p.max_pages + (s.len >> p.shift)] : kNone;
+}
 // Which of refs[at .. at + 15] are 0.  (Past the end the last sixteen are read, not one word after the other: 48
 // sequences of a pool of 16383 pages 12.3 -> 11.2 us with a trim.)
 __device__ inline uint32_t look(const Pages &p, uint32_t at) {
@@ -221,10 +225,46 @@ __device__ inline Plan plan_of(const Pages &p) {
   return {first, first + p.b + 1, first + p.b + 1 + segments(p.n_pages)};
 }
 
-// A sequence whose last page has other holders.
+// A sequence whose last page has `held` holders, more than itself.
 struct Sharer {
-  uint32_t seq, page, len, held, yes;
+  uint32_t seq, page, len, held, copies;
 };
+// Whether another sequence has a sharer's page, at the same place of its row.  Up to kNear sequences a wave of
+// the grow looks through them; of more kv4_others_kernel has noted it.  (One token each, every page held elsewhere too: 128
+// sequences 15.6 us, 129 13.0 with 3.7 of that kernel before; 1000, of which 50 are such, 34 looked up by the grow's
+// workgroup, 13.0 and 7.2 so.)
+constexpr uint32_t kNear = 128;
+__device__ inline bool has(const Pages &p, uint32_t j, const Sharer &s) {
+  const uint32_t i = j < p.b ? j : s.seq, c = s.len >> p.shift;
+  return p.table[(size_t)i * p.max_pages + c] == s.page && i != s.seq && pages_of(length(p, i), p.shift) > c;
+}
+__device__ inline uint32_t *others_have_of(const Pages &p) { return plan_of(p).first; }  // (until the plan is there)
+__device__ inline bool others_have(const Pages &p, const Sharer &s) {
+  if (p.b > kNear) return others_have_of(p)[s.seq];
+  bool found = false;
+#pragma unroll
+  for (uint32_t u = 0; u < kNear; u += 64) found |= has(p, u + (threadIdx.x & 63), s);
+  return __any(found);
+}
+// A wave per sequence, 256 others at a time from its neighbours on.  (What is read goes with the sharers times the
+// sequences: 256 prompts 4.1 us, 4096 sequences with 205 sharers 17, 16384 that all are 675.)
+__global__ __launch_bounds__(256) void kv4_others_kernel(Pages p, const uint32_t *__restrict__ add) {
+  const uint32_t lane = threadIdx.x & 63, i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Seq s = seq_of(p, add, i);
+  const uint32_t q = last_page(p, i, s);
+  if (q >= p.n_pages || p.refs[q] <= 1) return;  // (not asked for)
+  const Sharer own{i, q, s.len, 0, 0};
+  const uint32_t chunks = (p.b + 63) / 64;
+  bool found = false;
+  for (uint32_t k = 0; k < chunks && !found; k += 4) {
+    bool here = false;
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) here |= has(p, (i / 64 + k + u) % chunks * 64 + lane, own);
+    found = __any(here);
+  }
+  if (lane == 0) others_have_of(p)[i] = found;
+}
+
 // Up to so many of them find one another in LDS, at a cost that goes with their square; more through mark's six phases.  (A
 // step of as many beams: 40 8.6 / 10.8 us, 128 10.7 / 11.0, 192 12.1 / 11.4, 800 50 / 16; 48 sequences, two of them on kept
 // prompts' pages, 10.0 / 12.0.)
@@ -237,15 +277,17 @@ constexpr uint32_t kFew = 128;
 //  2. a tile's sums of the pages and rows asked for decide who grows; lengths and row offsets
 //  3. refs are looked through from page 0 for as many free pages as that takes, 16384 at a time
 //     (the first ones are asked for at the start: a page that is free then is so until it is given out)
-// Bound by latency, about ten dependent steps: 48 sequences of up to 5 tokens 7.9 us with the maps; as kPlan, 256
-// prompts of up to 4096 tokens, 4.2.
+// Bound by latency, about ten dependent steps: 48 sequences of up to 5 tokens 8.0 us with the maps and no copies asked for,
+// 8.6 with copies where no page has other holders, 9.6 where two are kept prompts'; as kPlan, 256 prompts of up to 4096
+// tokens, 4.2, 5.7 and 6.5.  A step of 40 beams on shared pages 8.7, of 512 20 (of which the look from page 0 through the
+// used ones of 67000 is a part).
 // kMaps (one tile): the rows' maps too.  kPlan: 3 is left to kv4_give_kernel, and the grid's other workgroups
 // note the free pages for it meanwhile (a page in use has a holder at every moment of 1 and 2).
 enum Grow { kPlain, kMaps, kPlan };
 template <Grow MODE>
 __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t *__restrict__ add, Rows r) {
   constexpr bool MAPS = MODE == kMaps;
-  __shared__ uint32_t list[MODE == kPlan ? kGrow * sizeof(Sharer) / 4 : kGrow * kScan], lds[2][kGrow / 64], asking;
+  __shared__ uint32_t list[MODE == kPlan ? kFew * sizeof(Sharer) / 4 : kGrow * kScan], lds[2][kGrow / 64], asking;
   __shared__ uint32_t offs[MAPS ? kGrow + 1 : 1], ends[MAPS ? kGrow : 1];
   const uint32_t tid = threadIdx.x, tiles = MAPS ? 1 : (p.b + kGrow - 1) / kGrow, mask = (1u << p.shift) - 1;
   if (MODE == kPlan && blockIdx.x) {
@@ -261,50 +303,10 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
     return;
   }
   const auto seq = [&](uint32_t i) { return seq_of(p, add, i); };
-  const auto last_page = [&](uint32_t i, const Seq &s) {  // the page that its next token goes to, if it has one
-    return s.add && (s.len & mask) ? p.table[(size_t)i * p.max_pages + (s.len >> p.shift)] : kNone;
-  };
   const uint32_t free = p.state[0];
   uint32_t is_free = MODE == kPlan ? 0 : look(p, tid * kScan);
 
-  // Whether another sequence than i has page q as number c of its own: a wave looks, 256 rows at a time from i's
-  // neighbours on.
   const uint32_t lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const auto another = [&](uint32_t i, uint32_t q, uint32_t c) {
-    const uint32_t chunks = (p.b + 63) / 64;
-    for (uint32_t k = 0; k < chunks; k += 4) {
-      uint32_t j[4], v[4];
-#pragma unroll
-      for (uint32_t u = 0; u < 4; ++u) {
-        j[u] = (i / 64 + k + u) % chunks * 64 + lane;
-        v[u] = p.table[(size_t)(j[u] < p.b ? j[u] : i) * p.max_pages + c];
-      }
-      bool found = false;
-#pragma unroll
-      for (uint32_t u = 0; u < 4; ++u)
-        found |= v[u] == q && j[u] < p.b && j[u] != i && pages_of(length(p, j[u]), p.shift) > c;
-      if (__any(found)) return true;
-    }
-    return false;
-  };
-  // The sequences of the threads with `mine` side by side in LDS, f(e, n) of each of the n by a wave, and what that says.
-  Sharer *sharers = reinterpret_cast<Sharer *>(list);
-  // (asking is 0)
-  const auto ask_of = [&](bool mine, const Sharer &own, auto f) {
-    uint32_t at = 0;
-    if (mine) {
-      at = atomicAdd(&asking, 1u);
-      sharers[at] = own;
-    }
-    __syncthreads();
-    const uint32_t n = asking;
-    for (uint32_t e = wave; e < n; e += kGrow / 64) {
-      const bool yes = f(e, n);
-      if (lane == 0) sharers[e].yes = yes;
-    }
-    __syncthreads();
-    return mine && sharers[at].yes;
-  };
 
   uint64_t copy = 0;
   if (r.copies) {
@@ -313,32 +315,42 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
     for (uint32_t t = 0; t < tiles; ++t) {
       const uint32_t i = t * kGrow + tid;
       const Seq s = seq(i);
-      const uint32_t q = last_page(i, s), held = q < p.n_pages ? p.refs[q] : 0;
+      const uint32_t q = last_page(p, i, s), held = q < p.n_pages ? p.refs[q] : 0;
       own = {i, q, s.len, held, 0};
       if (held > 1) shared |= 1ull << t;
     }
     if (tid == 0) asking = 0;
     const uint32_t some = __syncthreads_count(shared != 0);
     if (some && some <= kFew && tiles == 1) {  // a wave counts a sharer's page among the others
-      copy = ask_of(shared, own, [&](uint32_t e, uint32_t n) {
+      Sharer *sharers = reinterpret_cast<Sharer *>(list);
+      uint32_t mine = 0;
+      if (shared) {
+        mine = atomicAdd(&asking, 1u);
+        sharers[mine] = own;
+      }
+      __syncthreads();
+      for (uint32_t e = wave; e < some; e += kGrow / 64) {
         const Sharer s = sharers[e];
         uint32_t grow = 0;
         bool most = true;
-        for (uint32_t x = lane; x - lane < n; x += 64) {
-          const Sharer o = sharers[x < n ? x : e];
-          const bool same = x < n && o.page == s.page;
+        for (uint32_t x = lane; x - lane < some; x += 64) {
+          const Sharer o = sharers[x < some ? x : e];
+          const bool same = x < some && o.page == s.page;
           grow += __builtin_popcountll(__ballot(same));
           most &= !same || (o.len & mask) < (s.len & mask) || ((o.len & mask) == (s.len & mask) && o.seq <= s.seq);
         }
-        return grow < s.held ? !r.kept || another(s.seq, s.page, s.len >> p.shift) : !__all(most);
-      });
+        const bool copies = grow < s.held ? !r.kept || others_have(p, s) : !__all(most);
+        if (lane == 0) sharers[e].copies = copies;
+      }
+      __syncthreads();
+      copy = shared && sharers[mine].copies;
     } else if (some) {
       // through mark, which is 0 before and after: how many of a page's holders grow, then the longest of them
       const auto each = [&](uint64_t who, auto f) {
         for (uint32_t t = 0; t < tiles; ++t)
           if (who >> t & 1) {
             const uint32_t i = t * kGrow + tid;
-            f(t, i, last_page(i, seq(i)));
+            f(t, i, last_page(p, i, seq(i)));
           }
         __syncthreads();
       };
@@ -356,16 +368,8 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
       const uint64_t whole = shared & ~copy;  // of whose page all holders grow
       if (r.kept)
         for (uint32_t t = 0; t < tiles; ++t) {
-          const bool mine = copy >> t & 1;
           const uint32_t i = t * kGrow + tid;
-          if (tid == 0) asking = 0;
-          if (!__syncthreads_or(mine)) continue;
-          const Seq its = seq(i);
-          const bool yes = ask_of(mine, {i, last_page(i, its), its.len, 0, 0}, [&](uint32_t e, uint32_t) {
-            const Sharer s = sharers[e];
-            return another(s.seq, s.page, s.len >> p.shift);
-          });
-          if (mine && !yes) copy &= ~(1ull << t);
+          if (copy >> t & 1 && !others_have_of(p)[i]) copy &= ~(1ull << t);
         }
       if (__syncthreads_or(whole != 0)) {
         const auto tokens = [&](uint32_t i) { return length(p, i) & mask; };  // (at least one)
@@ -398,7 +402,7 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
     const uint32_t i = t * kGrow + tid;
     const Seq s = seq(i);
     const bool cp = copy >> t & 1;
-    const uint32_t src = cp ? last_page(i, s) : kNone, col = pages_of(s.len, p.shift);
+    const uint32_t src = cp ? last_page(p, i, s) : kNone, col = pages_of(s.len, p.shift);
     const uint32_t want = pages_of(s.len + s.add, p.shift) - col + cp;
     uint32_t ask[] = {want, s.add}, all[2], get[2], took_all[2];
     before(ask, lds, all);
@@ -589,6 +593,10 @@ extern "C" int madi_kv4_grow(const madi_kv4_pages *pages, const uint32_t *add, c
   if (int rc = ready(x)) return rc;
   const Rows r{rows->row_off, rows->copies, rows->row_seq, rows->row_pos, rows->slot, rows->m, rows->kept};
   const bool maps = m && (r.row_seq || r.row_pos || r.slot);
+  if (r.copies && r.kept && a.b > kNear) {
+    kv4_others_kernel<<<(a.b + 3) / 4, 256, 0, stream()>>>(a, add);
+    if (int rc = check_launch(what)) return rc;
+  }
   // Few rows: one workgroup.  More: the plan's launches, 3 us more, with the pages and maps over all CUs.  (Measured with
   // a trim, one workgroup against the plan: 48 sequences of 20 rows 11.7 / 14.4 us, of 80 20.8 / 14.4; 256 of 16
   // 17.0 / 18.2, of 64 29 / 21, of 256 82 / 21; 1024 of 4 27 / 33.)
