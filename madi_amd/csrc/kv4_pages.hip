@@ -48,7 +48,8 @@ __device__ inline void add_free(const Pages &p, int n) {
 // thread per column: the column's entries of all beams go through LDS, so that each is
 // read before one is written (in registers a column of 32 spilled).  Bound by latency: parents, lengths, entries, counts
 // one after the other; 64 groups of 8 beams with 1024 columns 5.4 us (12.3 with 256 threads a group, whose passes
-// follow one another), 8 groups of 5 with 7 4.4.
+// follow one another), 8 groups of 5 with 7 4.4, where no entry changes; where every beam's last pages do, 11.2 (18.2)
+// and 8.1: the counts' atomics, and the sum's.
 constexpr uint32_t kMaxBeams = 32, kForkLds = 32 << 10;
 __global__ __launch_bounds__(1024) void kv4_fork_kernel(Pages p, const uint32_t *__restrict__ parent, uint32_t ldp,
                                                          uint32_t beams) {
@@ -279,8 +280,8 @@ constexpr uint32_t kFew = 128;
 //     (the first ones are asked for at the start: a page that is free then is so until it is given out)
 // Bound by latency, about ten dependent steps: 48 sequences of up to 5 tokens 8.0 us with the maps and no copies asked for,
 // 8.6 with copies where no page has other holders, 9.6 where two are kept prompts'; as kPlan, 256 prompts of up to 4096
-// tokens, 4.2, 5.7 and 6.5.  A step of 40 beams on shared pages 8.7, of 512 20 (of which the look from page 0 through the
-// used ones of 67000 is a part).
+// tokens, 4.2, 5.7 and 6.5.  A step of 40 beams on shared pages 8.7, of 512 20 (of which the look from page 0 through
+// 36000 used ones is a part).
 // kMaps (one tile): the rows' maps too.  kPlan: 3 is left to kv4_give_kernel, and the grid's other workgroups
 // note the free pages for it meanwhile (a page in use has a holder at every moment of 1 and 2).
 enum Grow { kPlain, kMaps, kPlan };
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
           grow += __builtin_popcountll(__ballot(same));
           most &= !same || (o.len & mask) < (s.len & mask) || ((o.len & mask) == (s.len & mask) && o.seq <= s.seq);
         }
-        const bool copies = grow < s.held ? !r.kept || others_have(p, s) : !__all(most);
+        const bool copies = grow < s.held ? !r.kept || grow > 1 || others_have(p, s) : !__all(most);
         if (lane == 0) sharers[e].copies = copies;
       }
       __syncthreads();
@@ -361,15 +362,18 @@ __global__ __launch_bounds__(kGrow) void kv4_grow_kernel(Pages p, const uint32_t
       each(shared, [&](uint32_t, uint32_t, uint32_t q) {
         __hip_atomic_fetch_add(p.mark + q, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       });
+      uint64_t single = 0;  // of whose page one holder grows
       each(shared, [&](uint32_t t, uint32_t, uint32_t q) {
-        if (load(q) < p.refs[q]) copy |= 1ull << t;
+        const uint32_t n = load(q);
+        if (n < p.refs[q]) copy |= 1ull << t;
+        if (n == 1) single |= 1ull << t;
       });
       each(shared, clear);
       const uint64_t whole = shared & ~copy;  // of whose page all holders grow
       if (r.kept)
         for (uint32_t t = 0; t < tiles; ++t) {
           const uint32_t i = t * kGrow + tid;
-          if (copy >> t & 1 && !others_have_of(p)[i]) copy &= ~(1ull << t);
+          if (copy >> t & single >> t & 1 && !others_have_of(p)[i]) copy &= ~(1ull << t);
         }
       if (__syncthreads_or(whole != 0)) {
         const auto tokens = [&](uint32_t i) { return length(p, i) & mask; };  // (at least one)
@@ -598,7 +602,7 @@ extern "C" int madi_kv4_grow(const madi_kv4_pages *pages, const uint32_t *add, c
     if (int rc = check_launch(what)) return rc;
   }
   // Few rows: one workgroup.  More: the plan's launches, 3 us more, with the pages and maps over all CUs.  (Measured with
-  // a trim, one workgroup against the plan: 48 sequences of 20 rows 11.7 / 14.4 us, of 80 20.8 / 14.4; 256 of 16
+  // a trim and without copies, whose cost is the same in both, one workgroup against the plan: 48 sequences of 20 rows 11.7 / 14.4 us, of 80 20.8 / 14.4; 256 of 16
   // 17.0 / 18.2, of 64 29 / 21, of 256 82 / 21; 1024 of 4 27 / 33.)
   if (m <= 2048 + 8 * (a.b < kGrow ? a.b : kGrow)) {
     if (maps && b <= kGrow) kv4_grow_kernel<kMaps><<<1, kGrow, 0, stream()>>>(a, add, r);

@@ -178,6 +178,35 @@ def test_pages_of_many_tokens(kv4):
         assert (t.grow([0, 1, 1, 1])[:, 0] >= 0).tolist() == [False, True, True, False]
 
 
+@pytest.mark.parametrize("b,m", [(150, 150), (20, 40), (1030, 1030), (150, 9000)])
+def test_graph_replays_with_kept_prompts(kv4, b, m):
+    """A captured grow, replayed after other pages were held, with eager steps between."""
+    import madi_amd.q8 as q8
+    rng = np.random.default_rng(b)
+    t = Both(kv4, 3 * b, 16, b, 4, m)
+    t.grow(np.minimum(rng.integers(1, 3, b), m // b))
+    add = dev(np.ones(b))
+    torch.cuda.synchronize()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        q8.init(stream)
+        kv4.kvGrow(t.gpu, add)
+    q8.init()
+    for k in range(4):
+        used = np.flatnonzero(t.ref.refs)
+        t.hold(used[rng.random(len(used)) < 0.4])
+        if k % 2:
+            t.fork(rng.integers(0, 2, (b // 2, 2)), 2)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        expect = t.ref.grow(np.ones(b, int), m)
+        t.same()
+        for name, e in zip(("row_off", "copies", "row_seq", "row_pos", "slot"), expect):
+            np.testing.assert_array_equal(getattr(t.gpu, name).cpu().numpy(), e, err_msg=name)
+        t.grow((rng.random(b) < 0.5).astype(int))
+
+
 @pytest.fixture
 def cases():
     from perf import more_operators
