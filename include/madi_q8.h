@@ -436,7 +436,8 @@ size_t madi_kv4_attn_bytes(const madi_kv4 *cache, const madi_kv4_batch *batch, u
  * table serves every layer's) given out, shared and taken back by kernels, so that a
  * serving step needs nothing from the host.  refs[p] is how many table entries name
  * page p (0: free; what is held elsewhere counts too), state[0] the number of pages with
- * refs 0, state[1] how many sequences the last madi_kv4_grow left out.  mark is
+ * refs 0 (whoever holds pages elsewhere or gives them back keeps it so: by a larger number
+ * sequences grow without pages, by a smaller one pages stay unused), state[1] how many sequences the last madi_kv4_grow left out.  mark is
  * scratch, its first n_pages words zeros before the first call and after each.  Entries of a row past
  * its sequence's pages are 0xffffffff after a call that took the pages back; entries of n_pages or
  * more stand for pages that are not there and are counted nowhere.  The arrays must not

@@ -110,7 +110,7 @@ def beamGather(dst, src, parent, beams: int, lens=None) -> None:
     """Slot (g, i) of every state in dst becomes slot (g, parent[g][i]) of the state in
     src at the same place (src None, or the same tensors: in place); a parent that is no beam (-1) leaves it.
     dst, src: lists of tensors [groups * beams][rows][...], alike, each slot contiguous
-    (at most 32 a call go in one launch).  lens [groups * beams], int32: rows that the slot read
+    (32 go in one launch; more take several, each checked by itself before it).  lens [groups * beams], int32: rows that the slot read
     holds; the rows behind them are left as they were."""
     what, t = "beamGather", _torch()
     src = dst if src is None else src
