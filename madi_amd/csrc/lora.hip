@@ -79,7 +79,8 @@ __device__ inline uint32_t neighbours() {
 // A workgroup of 16 waves per row, wave w has ranks w, w + 16, ...: x rounded to f16 once, through LDS; the adapter's
 // rows S loads of 512 elements at a time, the next ones always on their way, the first before x is there.  (Loads past
 // the end of a row take its last elements: with a branch around each, every use waited for the newest load.)  Bound by
-// what a CU takes in, 50 GB/s: 40 rows of 5120 with rank 32 7.4 us (10.0 with branches), 8 of 1280 with 16 3.5.  Grid (m).
+// waits for memory: 40 rows of 5120 with rank 32 7.4 us (10.0 with branches), 340 KB into each of 40 CUs, whose waves wait
+// 55 % of their cycles (counters) and keep the vector pipes busy for a tenth; 8 of 1280 with 16 3.5.  Grid (m).
 constexpr uint32_t kStep = 512;
 template <int S>
 __global__ __launch_bounds__(1024) void lora_row_kernel(Adapters l, const float *__restrict__ in, uint32_t k,
@@ -164,9 +165,10 @@ __global__ __launch_bounds__(1024) void lora_row_kernel(Adapters l, const float 
 // Many rows: a workgroup of 16 waves per 16 rows, v_mfma_f32_16x16x32_f16 with the adapter's rows as the first
 // operand.  x goes through LDS in f16, kChunk elements of a row at a time (and to x16 where that is asked for); the
 // waves deal out the 16-row tiles of the rank (RT) and the chunk's steps of 32.  Each adapter of the rows takes a pass;
-// where CUs are left over, grid y of them deal the passes out.  Bound as the row kernel is: 2000 rows of 1280, 12
-// adapters of rank 64, 11.6 us (15.4 with branches around the loads and both passes of a tile with two adapters in one
-// workgroup).  Grid (m / 16, 1 to 4).
+// where CUs are left over, grid y of them deal the passes out.  Bound by waits for memory (57 % of the waves' cycles)
+// and by too few workgroups: 2000 rows of 1280, 12 adapters of rank 64, 11.6 us on 125 CUs, and a second adapter's pass on few
+// more (15.4 with branches around the loads and both passes of a tile with two adapters in one workgroup).  Grid (m / 16,
+// 1 to 4).
 constexpr uint32_t kTileWaves = 16, kChunk = 2048, kPitch = kChunk * 2 + 16;  // (rows 16 bytes off: other banks)
 template <int RT>
 __global__ __launch_bounds__(kTileWaves * 64) void lora_tile_kernel(Adapters l, const float *__restrict__ in, uint32_t m,

@@ -229,7 +229,8 @@ class Pages:
     row_seq, row_pos and slot [m] describe the new rows, and copies [b][3] the pages that
     kvCopy has to copy in every pool before they are stored.  state is [free pages,
     sequences that the last kvGrow left out]: whoever holds pages elsewhere (refs += 1) or gives them
-    back takes those that were free off state[0], and adds those that are now."""
+    back takes those that were free off state[0], and adds those that are now.
+    (So one Pages over its tensors: another's state would not follow.)"""
 
     def __init__(self, refs, table, lens, page: int, m: int | None = None):
         import torch
